@@ -337,6 +337,75 @@ int rai_hip_rope_tables(int dev, double theta, int32_t rot_dim, int32_t f64_powf
 int rai_hip_attention(int dev, const rai_hip_tensor *q, const rai_hip_tensor *k, const rai_hip_tensor *v,
                       double scale, int32_t causal, int32_t f32_scores, const rai_hip_tensor *out);
 
+/* --------------------------------- many requests over a paged 8-bit cache
+ *
+ * A program that serves requests of different lengths keeps their keys and values in pages of `page` tokens (16, 32, 64,
+ * 128 or 256), each page one request's, listed in order in that request's row of a block table.  One layer's cache is
+ *   k       u8  [pages, kv_heads, page, F]        v       u8  [pages, kv_heads, F, page]
+ *   k_scale f32 [pages, kv_heads]                 v_scale f32 [pages, kv_heads]
+ * contiguous, on 16 bytes; F is the head's features rounded up to a multiple of 16, at most 256, those behind the head's zero.
+ * A value is its code times its page's and head's scale.  Rows of a step are packed: request r's new tokens are rows
+ * starts[r] .. starts[r + 1] - 1, the last of its lens[r] tokens.  A step of a layer:
+ *   rai_hip_kv_plan (once a step), rai_hip_rope_positions on q and k, rai_hip_kv_append, rai_hip_kv_attention.
+ * None of them synchronises or needs to know a length on the host.  No counterpart in the reference (its models concatenate one
+ * sequence's cache, phi2.rs:233-243). */
+typedef enum rai_hip_kv_format {
+  RAI_KV_E4M3 = 0, /* 8-bit floating point, 4 bits of exponent, 3 of mantissa, largest 448, no infinities */
+  RAI_KV_INT8 = 1  /* whole numbers -127 .. 127 */
+} rai_hip_kv_format;
+
+/* Block tables and slots from request lengths.  Request r holds lens[r] tokens and is given add[r] more (0: it pauses), which may
+ * need pages: they are free_pages[taken[0]], free_pages[taken[0] + 1], ... in the order of the requests.
+ *   lens, add i64 [R]; free_pages u32 [F]; taken i64 [1]; tables u32 [R, M] (unit stride along M, any between rows)
+ *   out_tables  tables with the new pages entered; may be `tables` itself (nothing else is written then), no other output
+ *               may lie over an input
+ *   out_lens    lens + add          out_taken  taken + pages given
+ *   starts      i64 [R + 1], running sums of add
+ *   positions   i64 [N], each row's position in its request, -1 for rows behind the last request's
+ *   runs        u32 [4, W]: for each page that gets tokens its number, the first slot, the first row and how many; zeros behind
+ *               the last.  W is at least min(N, N / page + 2 R).
+ * A request is refused when its length is negative or past M * page, its rows past N, or the pages left are too few (counted in
+ * order: once one does not fit, later ones that need pages do not either).  It keeps its length, its rows' positions are -1, it has
+ * no runs, and the call counts as an index error (rai_hip_index_errors).  R is at most 4096. */
+int rai_hip_kv_plan(int dev, const rai_hip_tensor *lens, const rai_hip_tensor *add, const rai_hip_tensor *free_pages,
+                    const rai_hip_tensor *taken, const rai_hip_tensor *tables, int32_t page, const rai_hip_tensor *out_tables,
+                    const rai_hip_tensor *out_lens, const rai_hip_tensor *out_taken, const rai_hip_tensor *starts,
+                    const rai_hip_tensor *positions, const rai_hip_tensor *runs);
+
+/* Radians a position for rai_hip_rope_positions, f64 [rot / 2]: base^(-2 i / rot).  factor > 0: waves longer than original / low
+ * positions are stretched by it, those shorter than original / high kept, blended between (as rot_factor .. rot_original of
+ * rai_hip_hybrid_layer).  A program may fill such a tensor by any other rule. */
+int rai_hip_rope_frequencies(int dev, double base, double factor, double low, double high, double original, const rai_hip_tensor *out);
+/* Rotary embedding where every row has its own position: x [N, H, D] (bf16, f16 or f32; any strides between rows and heads),
+ * positions i64 [N], frequencies f64 [rot / 2], rot <= D.  Pair i of a head, features (i, i + rot / 2) or, interleaved,
+ * (2 i, 2 i + 1), turns by position * frequency (in 64 bits) and is multiplied by `magnitude`; features from rot on are copied.
+ * inverse != 0 turns back by the same angle, times magnitude: the gradient with respect to x of the gradient that x then is.
+ * Rounded once. */
+int rai_hip_rope_positions(int dev, const rai_hip_tensor *x, const rai_hip_tensor *positions, const rai_hip_tensor *frequencies,
+                           int32_t interleaved, int32_t inverse, double magnitude, const rai_hip_tensor *out);
+
+/* New keys and values [N, kv_heads, D] (bf16, f16 or f32; any strides between rows and heads) into the cache, in place, by the
+ * runs of rai_hip_kv_plan.  For each page and head that gets tokens the scale becomes 2^e, e the least for which the largest
+ * finite new magnitude is at most 448 (127) * 2^e, from -100 to 119 (121); where the run begins behind slot 0 the scale does not
+ * fall, and if it rises the page's earlier codes are rounded to it.  A run that begins at slot 0 forgets what the page held.
+ * Codes are rounded to nearest even; infinities become the largest code and NaN zero, as in rai_hip_cast to whole numbers.
+ * Slots behind a run are left as they are.  A run that names no page, or slots or rows that are not there, or a page that
+ * an earlier run of the call names too, is not stored and counts as an index error. */
+int rai_hip_kv_append(int dev, const rai_hip_tensor *new_k, const rai_hip_tensor *new_v, const rai_hip_tensor *runs, int32_t format,
+                      const rai_hip_tensor *k, const rai_hip_tensor *v, const rai_hip_tensor *k_scale, const rai_hip_tensor *v_scale);
+
+/* Scaled-dot-product attention of packed rows q [N, Hq, D] (bf16, f16 or f32; any strides between rows and heads) over the cache,
+ * Hq a multiple of kv_heads.  Row i of request r sits at position p = lens[r] - (starts[r + 1] - starts[r]) + i and sees keys
+ * 0 .. p, of them the last `window` where window > 0; a row that sees none gives zeros.  Scores, softmax and sums are in f32, out
+ * [N, Hq, D] contiguous in q's dtype; rows that belong to no request are left as they are.
+ *   tables u32 [R, M] (unit stride along M), starts i64 [R + 1] not falling, lens i64 [R] (after rai_hip_kv_plan: out_lens)
+ * Pages of a shared prefix may stand in many tables.  A page number that is not there hides its tokens, and counts as an index error, as
+ * does a length past M * page, which is cut to that.  Codes that are NaN (no rai_hip_kv_append writes one) may reach rows that do not see
+ * their token.  The cut of long contexts over blocks needs scratch, which grows with N * Hq and is the device's. */
+int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_hip_tensor *tables, const rai_hip_tensor *starts, const rai_hip_tensor *lens,
+                         int32_t format, const rai_hip_tensor *k, const rai_hip_tensor *v, const rai_hip_tensor *k_scale,
+                         const rai_hip_tensor *v_scale, double scale, int32_t window, const rai_hip_tensor *out);
+
 /* ------------------------------------------- decoder-only model drivers */
 
 typedef enum rai_hip_arch {

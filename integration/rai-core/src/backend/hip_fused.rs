@@ -10,6 +10,7 @@
 //!   rms_norm     rai-nn/src/rms_norm.rs:18-22, rai-models/src/llm/gemma.rs:42-54 (add_one)
 //!   rope         rai-models/src/llm/phi2.rs:66-77, qwen2.rs:60-71
 //!   attention    rai-models/src/llm/phi2.rs:244-262 (f32 scores), qwen2.rs:205-216
+//!   kv_plan, rope_positions, kv_append, kv_attention   many requests over a paged 8-bit cache (no counterpart)
 //!   sample_argmax examples/phi2/src/main.rs:29-50
 //!   Decoder      rai-models/src/llm/{phi2,qwen2,gemma,phi3}.rs `Model::{new, fwd, clear_kv_cache}` and the greedy
 //!                loop of examples/phi2/src/main.rs:72-95
@@ -56,6 +57,54 @@ pub fn rope(dev: c_int, x: &HipData, cos: &HipData, sin: &HipData, rot_dim: i32,
 #[allow(clippy::too_many_arguments)]
 pub fn attention(dev: c_int, q: &HipData, k: &HipData, v: &HipData, scale: f64, causal: bool, f32_scores: bool, out: &HipData) {
     check(unsafe { rai_hip_attention(dev, q.desc(), k.desc(), v.desc(), scale, causal as i32, f32_scores as i32, out.desc()) });
+}
+
+/// One layer's paged 8-bit cache (see `rai_hip_kv_append` in the header): `k`, `v` codes, a scale for each page and head.
+pub struct KvCache<'a> {
+    pub format: i32,
+    pub k: &'a HipData,
+    pub v: &'a HipData,
+    pub k_scale: &'a HipData,
+    pub v_scale: &'a HipData,
+}
+
+/// Pages and slots of a step's tokens from request lengths; `out_tables` may be `tables`.
+#[allow(clippy::too_many_arguments)]
+pub fn kv_plan(dev: c_int, lens: &HipData, add: &HipData, free_pages: &HipData, taken: &HipData, tables: &HipData, page: i32,
+               out_tables: &HipData, out_lens: &HipData, out_taken: &HipData, starts: &HipData, positions: &HipData, runs: &HipData) {
+    check(unsafe {
+        rai_hip_kv_plan(dev, lens.desc(), add.desc(), free_pages.desc(), taken.desc(), tables.desc(), page, out_tables.desc(),
+                        out_lens.desc(), out_taken.desc(), starts.desc(), positions.desc(), runs.desc())
+    });
+}
+
+pub fn rope_frequencies(dev: c_int, base: f64, factor: f64, low: f64, high: f64, original: f64, out: &HipData) {
+    check(unsafe { rai_hip_rope_frequencies(dev, base, factor, low, high, original, out.desc()) });
+}
+
+#[allow(clippy::too_many_arguments)]
+pub fn rope_positions(dev: c_int, x: &HipData, positions: &HipData, frequencies: &HipData, interleaved: bool, inverse: bool,
+                      magnitude: f64, out: &HipData) {
+    check(unsafe {
+        rai_hip_rope_positions(dev, x.desc(), positions.desc(), frequencies.desc(), interleaved as i32, inverse as i32, magnitude,
+                               out.desc())
+    });
+}
+
+pub fn kv_append(dev: c_int, new_k: &HipData, new_v: &HipData, runs: &HipData, c: &KvCache) {
+    check(unsafe {
+        rai_hip_kv_append(dev, new_k.desc(), new_v.desc(), runs.desc(), c.format, c.k.desc(), c.v.desc(), c.k_scale.desc(),
+                          c.v_scale.desc())
+    });
+}
+
+#[allow(clippy::too_many_arguments)]
+pub fn kv_attention(dev: c_int, q: &HipData, tables: &HipData, starts: &HipData, lens: &HipData, c: &KvCache, scale: f64, window: i32,
+                    out: &HipData) {
+    check(unsafe {
+        rai_hip_kv_attention(dev, q.desc(), tables.desc(), starts.desc(), lens.desc(), c.format, c.k.desc(), c.v.desc(),
+                             c.k_scale.desc(), c.v_scale.desc(), scale, window, out.desc())
+    });
 }
 
 /// `apply_repeat_penalty` + `sample_argmax` of the example binaries on a `[rows, vocab]` logits tensor.

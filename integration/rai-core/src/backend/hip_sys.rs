@@ -59,6 +59,8 @@ pub const RAI_BIN_LE: i32 = 11;
 pub const RAI_RED_SUM: i32 = 0;
 pub const RAI_RED_MAX: i32 = 1;
 pub const RAI_RED_MIN: i32 = 2;
+pub const RAI_KV_E4M3: i32 = 0;
+pub const RAI_KV_INT8: i32 = 1;
 pub const RAI_ARCH_PHI2: i32 = 0;
 pub const RAI_ARCH_QWEN2: i32 = 1;
 pub const RAI_ARCH_GEMMA: i32 = 2;
@@ -237,6 +239,11 @@ extern "C" {
     pub fn rai_hip_rope(dev: c_int, x: *const RaiHipTensor, cos: *const RaiHipTensor, sin: *const RaiHipTensor, rot_dim: i32, offset: i64, out: *const RaiHipTensor) -> c_int;
     pub fn rai_hip_rope_tables(dev: c_int, theta: f64, rot_dim: i32, f64_powf: i32, cos: *const RaiHipTensor, sin: *const RaiHipTensor) -> c_int;
     pub fn rai_hip_attention(dev: c_int, q: *const RaiHipTensor, k: *const RaiHipTensor, v: *const RaiHipTensor, scale: f64, causal: i32, f32_scores: i32, out: *const RaiHipTensor) -> c_int;
+    pub fn rai_hip_kv_plan(dev: c_int, lens: *const RaiHipTensor, add: *const RaiHipTensor, free_pages: *const RaiHipTensor, taken: *const RaiHipTensor, tables: *const RaiHipTensor, page: i32, out_tables: *const RaiHipTensor, out_lens: *const RaiHipTensor, out_taken: *const RaiHipTensor, starts: *const RaiHipTensor, positions: *const RaiHipTensor, runs: *const RaiHipTensor) -> c_int;
+    pub fn rai_hip_rope_frequencies(dev: c_int, base: f64, factor: f64, low: f64, high: f64, original: f64, out: *const RaiHipTensor) -> c_int;
+    pub fn rai_hip_rope_positions(dev: c_int, x: *const RaiHipTensor, positions: *const RaiHipTensor, frequencies: *const RaiHipTensor, interleaved: i32, inverse: i32, magnitude: f64, out: *const RaiHipTensor) -> c_int;
+    pub fn rai_hip_kv_append(dev: c_int, new_k: *const RaiHipTensor, new_v: *const RaiHipTensor, runs: *const RaiHipTensor, format: i32, k: *const RaiHipTensor, v: *const RaiHipTensor, k_scale: *const RaiHipTensor, v_scale: *const RaiHipTensor) -> c_int;
+    pub fn rai_hip_kv_attention(dev: c_int, q: *const RaiHipTensor, tables: *const RaiHipTensor, starts: *const RaiHipTensor, lens: *const RaiHipTensor, format: i32, k: *const RaiHipTensor, v: *const RaiHipTensor, k_scale: *const RaiHipTensor, v_scale: *const RaiHipTensor, scale: f64, window: i32, out: *const RaiHipTensor) -> c_int;
     pub fn rai_hip_decoder_create(dev: c_int, cfg: *const RaiHipDecoderConfig, out: *mut *mut RaiHipDecoder) -> c_int;
     pub fn rai_hip_decoder_destroy(dec: *mut RaiHipDecoder) -> c_int;
     pub fn rai_hip_decoder_create_latent(dev: c_int, cfg: *const RaiHipLatentConfig, layers: *const RaiHipLatentLayer, out: *mut *mut RaiHipDecoder) -> c_int;

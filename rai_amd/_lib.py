@@ -25,6 +25,7 @@ REDUCE = {"sum": 0, "max": 1, "min": 2}
 ARCH = {"phi2": 0, "qwen2": 1, "gemma": 2, "phi3": 3, "lelitar": 4, "bezadra": 5}
 MLP_KIND = {"none": 0, "dense": 1, "moe": 2}
 MIXER = {"attention": 0, "channel_delta": 1}
+KV_FORMAT = {"e4m3": 0, "int8": 1}
 
 
 class RaiHipError(RuntimeError):
@@ -142,6 +143,11 @@ PROTOTYPES = {
     "rai_hip_rope": [C.c_int, _TP, _TP, _TP, _i32, _i64, _TP],
     "rai_hip_rope_tables": [C.c_int, _dbl, _i32, _i32, _TP, _TP],
     "rai_hip_attention": [C.c_int, _TP, _TP, _TP, _dbl, _i32, _i32, _TP],
+    "rai_hip_kv_plan": [C.c_int, _TP, _TP, _TP, _TP, _TP, _i32, _TP, _TP, _TP, _TP, _TP, _TP],
+    "rai_hip_rope_frequencies": [C.c_int, _dbl, _dbl, _dbl, _dbl, _dbl, _TP],
+    "rai_hip_rope_positions": [C.c_int, _TP, _TP, _TP, _i32, _i32, _dbl, _TP],
+    "rai_hip_kv_append": [C.c_int, _TP, _TP, _TP, _i32, _TP, _TP, _TP, _TP],
+    "rai_hip_kv_attention": [C.c_int, _TP, _TP, _TP, _TP, _i32, _TP, _TP, _TP, _TP, _dbl, _i32, _TP],
     "rai_hip_decoder_create": [C.c_int, C.POINTER(DecoderConfig), C.POINTER(_vp)],
     "rai_hip_decoder_create_latent": [C.c_int, C.POINTER(LatentConfig), C.POINTER(LatentLayer), C.POINTER(_vp)],
     "rai_hip_decoder_create_hybrid": [C.c_int, C.POINTER(HybridConfig), C.POINTER(HybridLayer), C.POINTER(_vp)],

@@ -8,10 +8,11 @@ definitions under rai-core/src/ops/.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 
-from ._lib import BINARY, DTYPE_BY_NAME, REDUCE, U8, U32, UNARY, call
+from ._lib import BINARY, DTYPE_BY_NAME, F64, I64, REDUCE, U8, U32, UNARY, call
 from .hip import HipTensor
 
 
@@ -264,4 +265,38 @@ def attention(q, k, v, scale, causal, f32_scores):
     b, hq, s, d = q.shape
     out = HipTensor.empty((b, s, hq * d), q.dtype, q.dev)
     call("rai_hip_attention", q.dev, _d(q), _d(k), _d(v), float(scale), int(causal), int(f32_scores), _d(out))
+    return out
+
+
+# ---------------------------------------------------------------- many requests over a paged cache (see kv_cache.py)
+class KvPlan(NamedTuple):
+    """What a step needs of rai_hip_kv_plan, all on the device."""
+    lens: HipTensor        # i64 [requests], the new tokens included
+    taken: HipTensor       # i64 [1]
+    starts: HipTensor      # i64 [requests + 1]
+    positions: HipTensor   # i64 [rows]
+    runs: HipTensor        # u32 [4, pieces]
+
+
+def kv_plan(lens, add, free_pages, taken, tables, page, rows):
+    """rai_hip_kv_plan: pages, positions and slots of a step's `rows` new tokens, add[r] of request r; new pages are entered
+    into `tables` in place."""
+    r, dev = tables.shape[0], tables.dev
+    plan = KvPlan(HipTensor.empty((r,), I64, dev), HipTensor.empty((1,), I64, dev), HipTensor.empty((r + 1,), I64, dev), HipTensor.empty((rows,), I64, dev),
+                  HipTensor.empty((4, min(rows, rows // page + 2 * r)), U32, dev))
+    call("rai_hip_kv_plan", dev, _d(lens), _d(add), _d(free_pages), _d(taken), _d(tables), int(page), _d(tables), *map(_d, plan))
+    return plan
+
+
+def rope_frequencies(rot_dim, base, factor=0.0, low=1.0, high=4.0, original=8192.0, dev=0):
+    """rai_hip_rope_frequencies: radians a position of each pair, f64 [rot_dim / 2]; factor > 0 stretches the long waves."""
+    out = HipTensor.empty((rot_dim // 2,), F64, dev)
+    call("rai_hip_rope_frequencies", dev, float(base), float(factor), float(low), float(high), float(original), _d(out))
+    return out
+
+
+def rope_positions(x, positions, frequencies, interleaved=False, inverse=False, magnitude=1.0):
+    """rai_hip_rope_positions: x [rows, heads, features], each row turned by its own position.  inverse: the gradient."""
+    out = HipTensor.empty(x.shape, x.dtype, x.dev)
+    call("rai_hip_rope_positions", x.dev, _d(x), _d(positions), _d(frequencies), int(interleaved), int(inverse), float(magnitude), _d(out))
     return out
