@@ -229,7 +229,7 @@ struct KvAppendArgs {
   const uint32_t *runs;
   int64_t N, W;
   int D;                         // the rows' features; those up to c.features are zero in the cache
-  int heads_per_block;
+  int rounds;                    // units a wave (or block) does in turn
   unsigned long long *errors;
 };
 
@@ -259,64 +259,217 @@ template <int FMT> __device__ __forceinline__ float kv_clamp(float x) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// One wave for each run, head and side (keys or values): the largest finite new magnitude, the scale 2^e that holds it (and what
-// the page holds already, whose codes are taken to the new scale where it is another), the new codes.  Scales are powers of two, so
-// a code's value over the old scale is exact and one in e4m3 is not rounded again unless it falls below the normal numbers.
-// A wave owns its page and head alone: a run whose page an earlier run of the call names is refused.
-template <typename T, int FMT>
+// V features of a row as they are read; those from D on are zero.
+template <typename T, bool VEC, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) KvPack { T v[V]; };
+template <typename T, bool VEC, int V> __device__ __forceinline__ KvPack<T, VEC, V> kv_load(const T *src, uint32_t d, uint32_t D) {
+  KvPack<T, VEC, V> p;
+  if constexpr (VEC) {
+    memset(&p, 0, sizeof(p));
+    if (d < D) p = *reinterpret_cast<const KvPack<T, VEC, V> *>(src + d);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      memset(&p.v[j], 0, sizeof(T));
+      if (d + j < D) p.v[j] = src[d + j];
+    }
+  }
+  return p;
+}
+// Keeps what was read in the registers as it is: widened copies of it would take twice as many.
+template <typename P> __device__ __forceinline__ void kv_keep(P &p) {
+  struct Words { uint32_t w[sizeof(P) / 4]; } x = __builtin_bit_cast(Words, p);
+#pragma unroll
+  for (size_t i = 0; i < sizeof(P) / 4; ++i) asm volatile("" : "+v"(x.w[i]));
+  p = __builtin_bit_cast(P, x);
+}
+template <typename T> __device__ __forceinline__ float finite_size(const T &v) {
+  const float x = fabsf((float)Scalar<T>::load(&v));
+  return x < INFINITY ? x : 0.f;
+}
+template <int FMT> __device__ __forceinline__ uint32_t kv_codes4(float a, float b, float c, float d) {
+  typedef KvFormat<FMT> Fm;
+  return Fm::code2(kv_clamp<FMT>(a), kv_clamp<FMT>(b)) | Fm::code2(kv_clamp<FMT>(c), kv_clamp<FMT>(d)) << 16;
+}
+// Four codes to another scale.
+template <int FMT> __device__ __forceinline__ uint32_t kv_rescale4(uint32_t x, float ratio) {
+  typedef KvFormat<FMT> Fm;
+  return kv_codes4<FMT>(Fm::value(x & 0xff) * ratio, Fm::value(x >> 8 & 0xff) * ratio, Fm::value(x >> 16 & 0xff) * ratio, Fm::value(x >> 24) * ratio);
+}
+
+// A unit is a run's keys or values of one head: their largest finite magnitude, the scale 2^e that holds it (and what the page holds already, whose
+// codes are taken to the new scale where it is another), the codes.  Scales are powers of two, so a code's value over the old
+// scale is exact and one in e4m3 is not rounded again unless it falls below the normal numbers.
+// WAVES waves share a unit: one for pages of up to 4096 values, four beyond.  Keys go eight features of a token to a thread; of the
+// values, which lie transposed, a wave takes sixteen tokens and a thread two features of them, so that it reads four (f32: eight) bytes of each token and
+// writes whole 16-byte pieces of both features, without a trip through LDS.  What the first pass read stays in registers where a thread has
+// no more than four packs of keys or one piece of values, and is read again from the caches otherwise.
+// A unit owns its page and head alone: a run whose page an earlier run of the call names is refused.
+template <typename T, int FMT, bool VEC, int WAVES>
 __global__ void __launch_bounds__(256) k_kv_append(KvAppendArgs a) {
   typedef KvFormat<FMT> Fm;
-  const int lane = threadIdx.x & 63, w = blockIdx.x;
+  typedef KvPack<T, VEC, 8> Eight;
+  typedef KvPack<T, VEC, 2> Two;
+  constexpr int HELD = 4, LANES = 64 * WAVES;
+  __shared__ float tops[4];
+  const int w = blockIdx.x;
   const uint32_t page = a.runs[w], at = a.runs[a.W + w], row = a.runs[2 * a.W + w], count = a.runs[3 * a.W + w];
   if (count == 0) return;
-  bool bad = page >= a.c.pages || at >= (uint32_t)a.c.page || count > a.c.page - at || row >= a.N || count > a.N - row;
-  for (int64_t i = lane; i < w && !bad; i += 64) bad = a.runs[i] == page && a.runs[3 * a.W + i] != 0;
-  if (__any(bad)) {
+  if (page >= a.c.pages || at >= (uint32_t)a.c.page || count > a.c.page - at || row >= a.N || count > a.N - row) {
     if (blockIdx.y == 0 && threadIdx.x == 0) atomicAdd(a.errors, 1ull);
     return;
   }
-  const int units = 2 * a.heads_per_block, B = a.c.page, DC = a.c.features, D = a.D;
-  for (int u = threadIdx.x >> 6; u < units; u += 4) {
-    const int h = blockIdx.y * a.heads_per_block + (u >> 1), side = u & 1;
-    if (h >= a.c.heads) break;
-    const T *src = (const T *)a.src[side] + (int64_t)row * a.row[side] + (int64_t)h * a.head[side];
-    const int64_t ph = (int64_t)page * a.c.heads + h;
+  bool again = false;   // an earlier run has the page; asked for ahead of the values, answered behind them
+  for (int64_t i = threadIdx.x; i < w; i += 256)
+    if (a.runs[i] == page && a.runs[3 * a.W + i] != 0) again = true;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = threadIdx.x % LANES, B = a.c.page;
+  const uint32_t F = a.c.features, D = a.D, packs = F / 8, items = count * packs;        // of keys
+  const int piece0 = at / 16 + wave % WAVES, pieces = (at + count - 1) / 16 + 1;         // of values: pieces of 16 slots, this wave's first
+  for (int g = 0; g < a.rounds; ++g) {
+    const int unit = (blockIdx.y * a.rounds + g) * (4 / WAVES) + wave / WAVES, h = unit >> 1, side = unit & 1;
+    if (g > 0 && h >= a.c.heads) break;   // (in the first round every wave comes to the barrier)
+    const bool live = h < a.c.heads;
+    const int64_t stride = a.row[side], ph = (int64_t)page * a.c.heads + h;
+    const T *const src = (const T *)a.src[side] + (int64_t)row * stride + (int64_t)h * a.head[side];
     float *const scale = (side ? a.c.v_scale : a.c.k_scale) + ph;
-    uint8_t *const codes = (side ? a.c.v : a.c.k) + ph * B * DC;
-    float largest = 0.f;
-    for (uint32_t s = 0; s < count; ++s)
-      for (int d = lane; d < D; d += 64) {
-        const float x = fabsf((float)Scalar<T>::load(src + s * a.row[side] + d));
-        if (x < INFINITY) largest = fmaxf(largest, x);
+    uint8_t *const codes = (side ? a.c.v : a.c.k) + ph * B * F;
+    const float s_old = at > 0 && live ? *scale : 0.f;
+
+    Eight keys[HELD];
+    Two values[16];
+    float top = 0.f;
+    auto key_pack = [&](uint32_t e) __attribute__((always_inline)) {
+      const uint32_t s = e / packs;
+      return kv_load<T, VEC, 8>(src + s * stride, (e - s * packs) * 8, D);
+    };
+    // Sixteen tokens of features d and d + 1; slots of the piece without a new token repeat the nearest one, which changes no maximum.
+    auto value_piece = [&](int p, uint32_t d, Two *out) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) out[j] = kv_load<T, VEC, 2>(src + min(max(16 * p + j - (int)at, 0), (int)count - 1) * stride, d, D);
+    };
+    if (!live) {
+    } else if (side == 0) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) keys[i] = key_pack(min((uint32_t)(t + i * LANES), items - 1));
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_size(keys[i].v[j]));
+      for (uint32_t e = t + HELD * LANES; e < items; e += LANES) {
+        const Eight x = key_pack(e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_size(x.v[j]));
       }
-    largest = wave_max(largest);
+    } else {
+      if (piece0 < pieces) value_piece(piece0, 2 * lane, values);
+      if (piece0 < pieces)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, finite_size(values[j].v[0])), finite_size(values[j].v[1]));
+      for (int p = piece0; p < pieces; p += WAVES)
+        for (uint32_t d0 = p == piece0 ? 128 : 0; d0 < F; d0 += 128) {
+          Two x[16];
+          value_piece(p, d0 + 2 * lane, x);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(fmaxf(top, finite_size(x[j].v[0])), finite_size(x[j].v[1]));
+        }
+    }
+    top = wave_max(top);
+    if (WAVES == 4 && lane == 0) tops[wave] = top;
+    if (g == 0) {
+      if (__syncthreads_or(again)) {
+        if (blockIdx.y == 0 && threadIdx.x == 0) atomicAdd(a.errors, 1ull);
+        return;
+      }
+      if (!live) return;
+    } else if (WAVES == 4) {
+      __syncthreads();
+    }
+    if constexpr (WAVES == 4) {
+      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      __syncthreads();   // (tops serves the next unit; and every thread has read the old scale)
+    }
     int ex = kKvLeastExp;
-    if (largest > 0.f) {
+    if (top > 0.f) {
       int x;
-      const float m = frexpf(largest, &x);
+      const float m = frexpf(top, &x);
       ex = min(max(Fm::exponent(m, x), kKvLeastExp), Fm::kMostExp);
     }
-    float s_new = power_of_two(ex);
-    if (at > 0) {
-      const float s_old = *scale;
-      if (s_old >= s_new) s_new = s_old;
-      else {
-        const float ratio = s_old / s_new;
-        for (uint32_t e = lane; e < at * DC; e += 64) {
-          const uint32_t s = side ? e % at : e / DC, d = side ? e / at : e % DC;
-          uint8_t *p = codes + (side ? d * B + s : s * DC + d);
-          *p = (uint8_t)Fm::code2(kv_clamp<FMT>(Fm::value(*p) * ratio), 0.f);
+    if (side == 0) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) kv_keep(keys[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) kv_keep(values[j]);
+    }
+    const float s_own = power_of_two(ex), s_new = s_old >= s_own ? s_old : s_own, inverse = 1.f / s_new, ratio = s_old / s_new;
+    const bool rescale = at > 0 && s_old != s_new;
+    if (t == 0) *scale = s_new;
+    auto number = [&](const T &v) __attribute__((always_inline)) { return (float)Scalar<T>::load(&v) * inverse; };
+    if (side == 0) {
+      auto store = [&](uint32_t e, const Eight &x) __attribute__((always_inline)) {
+        *reinterpret_cast<uint2 *>(codes + at * F + 8 * e) = make_uint2(kv_codes4<FMT>(number(x.v[0]), number(x.v[1]), number(x.v[2]), number(x.v[3])),
+                                                                        kv_codes4<FMT>(number(x.v[4]), number(x.v[5]), number(x.v[6]), number(x.v[7])));
+      };
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (t + i * LANES < items) store(t + i * LANES, keys[i]);
+      for (uint32_t e = t + HELD * LANES; e < items; e += LANES) store(e, key_pack(e));
+      if (rescale)
+        for (uint32_t e = t; e < at * F / 16; e += LANES) {
+          uint4 *const p = reinterpret_cast<uint4 *>(codes) + e, x = *p;
+          *p = make_uint4(kv_rescale4<FMT>(x.x, ratio), kv_rescale4<FMT>(x.y, ratio), kv_rescale4<FMT>(x.z, ratio), kv_rescale4<FMT>(x.w, ratio));
         }
-      }
+    } else {
+      auto store = [&](int p, uint32_t d, const Two *x) __attribute__((always_inline)) {
+        if (d >= F) return;
+        const int first = (int)at - 16 * p, behind = first + (int)count;   // new tokens are slots first .. behind - 1 of the piece
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t c[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) c[j] = kv_codes4<FMT>(number(x[4 * j].v[i]), number(x[4 * j + 1].v[i]), number(x[4 * j + 2].v[i]), number(x[4 * j + 3].v[i]));
+          uint4 *const dst = reinterpret_cast<uint4 *>(codes + (d + i) * B + 16 * p);
+          if (first > 0 || behind < 16) {
+            const uint4 was = *dst;
+            const uint32_t old[4] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int lo = min(max(first - 4 * j, 0), 4), hi = min(max(behind - 4 * j, 0), 4);
+              const uint32_t before = lo == 4 ? 0xffffffffu : (1u << 8 * lo) - 1, upto = hi == 4 ? 0xffffffffu : (1u << 8 * hi) - 1;
+              const uint32_t kept = rescale ? kv_rescale4<FMT>(old[j], ratio) : old[j];
+              c[j] = (kept & before) | (c[j] & upto & ~before) | (old[j] & ~upto & ~before);
+            }
+          }
+          *dst = make_uint4(c[0], c[1], c[2], c[3]);
+        }
+      };
+      if (piece0 < pieces) store(piece0, 2 * lane, values);
+      for (int p = piece0; p < pieces; p += WAVES)
+        for (uint32_t d0 = p == piece0 ? 128 : 0; d0 < F; d0 += 128) {
+          Two x[16];
+          value_piece(p, d0 + 2 * lane, x);
+          store(p, d0 + 2 * lane, x);
+        }
+      if (rescale)   // whole pieces before the run's first
+        for (uint32_t e = t; e < at / 16 * F; e += LANES) {
+          const uint32_t p = e / F, d = e - p * F;
+          uint4 *const dst = reinterpret_cast<uint4 *>(codes + d * B + 16 * p), x = *dst;
+          *dst = make_uint4(kv_rescale4<FMT>(x.x, ratio), kv_rescale4<FMT>(x.y, ratio), kv_rescale4<FMT>(x.z, ratio), kv_rescale4<FMT>(x.w, ratio));
+        }
     }
-    const float inverse = 1.f / s_new;
-    for (uint32_t e = lane; e < count * DC; e += 64) {
-      const uint32_t s = side ? e % count : e / DC, d = side ? e / count : e % DC;
-      const float x = d < (uint32_t)D ? (float)Scalar<T>::load(src + s * a.row[side] + d) : 0.f;
-      codes[side ? d * B + at + s : (at + s) * DC + d] = (uint8_t)Fm::code2(kv_clamp<FMT>(x * inverse), 0.f);
-    }
-    if (lane == 0) *scale = s_new;
   }
+}
+
+template <typename T, int FMT> static void launch_kv_append(hipStream_t st, KvAppendArgs a, bool vec) {
+  const bool wide = a.c.page * a.c.features > 4096;
+  const int per_block = wide ? 1 : 4, groups = (2 * a.c.heads + per_block - 1) / per_block;
+  // A block looks once for its page among the runs before its own; where runs are many it then does several units' work.
+  int64_t rounds = a.W * groups / 4096;
+  a.rounds = (int)(rounds < 1 ? 1 : rounds < groups ? rounds : groups);
+  const dim3 grid((unsigned)a.W, (unsigned)((groups + a.rounds - 1) / a.rounds));
+  if (wide && vec) hipLaunchKernelGGL((k_kv_append<T, FMT, true, 4>), grid, dim3(256), 0, st, a);
+  else if (wide) hipLaunchKernelGGL((k_kv_append<T, FMT, false, 4>), grid, dim3(256), 0, st, a);
+  else if (vec) hipLaunchKernelGGL((k_kv_append<T, FMT, true, 1>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_kv_append<T, FMT, false, 1>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace rai
@@ -423,12 +576,15 @@ extern "C" int rai_hip_kv_append(int dev, const rai_hip_tensor *new_k, const rai
   a.row[1] = new_v->stride[0]; a.head[1] = new_v->stride[1];
   a.runs = (const uint32_t *)base_ptr(runs);
   a.errors = index_error_counter(dev);
-  a.heads_per_block = 2;
-  const dim3 grid((unsigned)a.W, (unsigned)((a.c.heads + a.heads_per_block - 1) / a.heads_per_block));
+  const int64_t es = (int64_t)dtype_size(new_k->dtype);
+  auto aligned = [&](const rai_hip_tensor *t) {
+    return (uintptr_t)base_ptr(t) % 16 == 0 && (N == 1 || t->stride[0] * es % 16 == 0) && (a.c.heads == 1 || t->stride[1] * es % 16 == 0);
+  };
+  const bool vec = D % 8 == 0 && aligned(new_k) && aligned(new_v);
 #define KV_APPEND(T)                                                                                              \
   do {                                                                                                            \
-    if (format == RAI_KV_E4M3) hipLaunchKernelGGL((k_kv_append<T, RAI_KV_E4M3>), grid, dim3(256), 0, st, a);      \
-    else hipLaunchKernelGGL((k_kv_append<T, RAI_KV_INT8>), grid, dim3(256), 0, st, a);                            \
+    if (format == RAI_KV_E4M3) launch_kv_append<T, RAI_KV_E4M3>(st, a, vec);                                      \
+    else launch_kv_append<T, RAI_KV_INT8>(st, a, vec);                                                            \
   } while (0)
   if (new_k->dtype == RAI_BF16) KV_APPEND(bf16_raw);
   else if (new_k->dtype == RAI_F16) KV_APPEND(f16_raw);
