@@ -21,15 +21,26 @@ struct KvAttnArgs {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   int64_t pages;
-  int R, Hq, Hkv, G, D, features, page_shift, window;
-  int q_aligned, out_aligned;
+  int dev, R, Hq, Hkv, G, D, features, page_shift, window;
   float scale_log2;              // scale * log2(e)
-  int splits, least;             // parts of a context, and steps of a part at least
+  double per_group;              // 1 / G
+  int reach;                     // keys that the oldest token of a tile sees, at most
   int which;                     // requests served: 0 all, 1 those of up to 16 columns, 2 the others
-  float *part;                   // [N * Hq][splits][features] sums, then their maxima and sums of weights
-  float *part_m, *part_l;
-  int *parts;                    // [N * Hq]: how many of `splits` there are
+  int each;                      // sixteenths of a key that a tile sees more than the one before it
+  double per_worker;             // 1 / workers
+  int workers;                   // of a key head, each with an even share of the steps; 0: a worker to a tile
+  int least;                     // steps of a share at least
+  float *part;                   // [Hkv * workers][2][columns of a tile][features] sums of a share's first and last tile
+  float *part_m, *part_l;        // their maxima and sums of weights
+  struct KvJoin *join;           // [Hkv * workers]
   unsigned long long *errors;
+};
+
+// The tile whose last part is a worker's first: workers first .. the worker itself have its parts.
+struct KvJoin {
+  int first;                     // -1: none
+  int place;                     // which of the first worker's two parts
+  int start, column, columns;    // the tile's request's first row, its first column and how many it has
 };
 
 // Eight codes as the eight bf16 of a fragment: every e4m3 value and every whole number up to 127 is a bf16.
@@ -49,6 +60,12 @@ template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, u
     }
   }
   return u.v;
+}
+
+// ONCE: read by one tile alone, so not to be kept in the L2.
+template <bool ONCE> __device__ __forceinline__ kv_u32x4 fetch(const uint8_t *p) {
+  const kv_u32x4 *q = reinterpret_cast<const kv_u32x4 *>(p);
+  return ONCE ? __builtin_nontemporal_load(q) : *q;
 }
 
 // How many bf16 hold a value of type T: products with codes are then exact, so f16 and f32 rows lose nothing on the bf16 matrix instructions.
@@ -88,388 +105,631 @@ __device__ __forceinline__ float column_sum(float v) { return column_fold(v, [](
 constexpr float kNoScore = -3.402823466e38f;   // a running maximum before the first key
 constexpr int kStep = 64;                      // keys of a step
 
+// Blocks of a kernel that a CU holds.
+constexpr int kv_blocks(int vt, int nc) { return nc > 1 || vt > 8 ? 1 : vt > 5 ? 2 : 3; }
+// Contexts of up to so many steps are not shared between workers.
+constexpr int kv_alone(int kw) { return kw == 1 ? 8 : 16; }
+constexpr int kv_least(int kw) { return kw == 1 ? 2 : 8; }
+
+// How the work of a key head is dealt out.  A tile of a request is as long as the keys that its last row sees, which grows evenly from tile to
+// tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1).
+constexpr int kUnits = 16 * kStep;   // of a step
+struct KvRequest {
+  int start, n, tiles;           // first row, new tokens
+  int len, first;                // length, cut to its table's; position of the first new token
+};
+__device__ __forceinline__ int64_t kv_base(const KvAttnArgs &a, const KvRequest &q) { return 16ll * min(max(q.len - q.n, 0), a.reach); }
+__device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return kv_base(a, q) + (int64_t)a.each * (tile + 1); }
+// of the tiles before `tile`
+__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return tile * kv_base(a, q) + a.each * (tile * (tile + 1) / 2); }
+
+template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, int r) {
+  KvRequest q;
+  const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), said = a.lens[r], most = a.M << a.page_shift;
+  q.start = (int)start;
+  q.n = (int)(min(max(a.starts[r + 1], start), a.N) - start);
+  q.len = (int)min(max(said, (int64_t)0), most);
+  q.first = (int)min(max(said, -(1ll << 30)), most) - q.n;
+  const int columns = q.n * a.G;
+  q.tiles = a.which == 1 ? columns > 0 && columns <= 16 : a.which == 2 && columns <= 16 ? 0 : (columns + QT - 1) / QT;
+  return q;
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
 // The columns of a request and key head are its new tokens times the query heads of the group, G to a token; a tile is 16 NC of them.  A
 // step is 64 keys:
 //     S^T = K . Q^T   (four tiles of 16 keys x 16 columns),      O^T = V^T . P^T   (VT tiles of 16 features x 16 columns)
 // on v_mfma_f32_16x16x32_bf16.  Row 4 g + r of score tile t is key 16 g + 4 t + r of the step, so that the lane group g (lanes 16 g ..) holds
 // the scores of sixteen neighbouring keys, which are the 16 bytes that it loads of a feature of V: the weights are the second product's
 // fragments as they lie in registers, and every load of the cache is 16 bytes a lane, straight to registers.  Sixteen keys lie in one
-// page, so a lane group has one page and one scale of keys and of values: scores and weights are multiplied by them.
-// KW waves share a tile's steps in turn and merge through LDS; with KW = 1 a wave has a tile to itself and blocks are four of them.
+// page, so a lane group has one page and one scale of keys and of values; both go into the exponent: with x = s ks and y = x + log2(vs),
+// exp2(y - m) is the weight times vs, and the sum of sixteen of them over vs is their share of the softmax's.
+// KW waves share a tile's steps in turn and merge through LDS; with KW = 1 a wave is a worker by itself and blocks are four of them.
 template <typename T, int FMT, int VT, int NC, int KW>
 __global__ void __launch_bounds__(256, NC * VT <= 8 ? 2 : 1) k_kv_attention(KvAttnArgs a) {
   constexpr int TERMS = KvTerms<T>::n, QT = 16 * NC, KL = VT / 4, KR = VT % 4;   // 16-byte loads of a key's features; features left
   constexpr int KS = 2 * KL + (KR == 0 ? 0 : KR == 3 ? 2 : 1);                     // products along the features
   constexpr int KN = KL + (KR == 3);                                               // whole 16-byte loads
   constexpr bool TAIL = KR == 1 || KR == 2;                                        // and one of 8 bytes
+  constexpr int WPB = 4 / KW;                                                      // workers of a block
+  constexpr bool HOIST = NC > 1 && VT <= 8 && TERMS == 1;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t slot = KW == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
-  const int kvh = blockIdx.y;
+  // Blocks go to the XCDs in turn: each gets neighbouring workers, whose keys are often the same.
+  const int blocks = gridDim.x * gridDim.y, linear = blockIdx.y * gridDim.x + blockIdx.x;
+  const int place = blocks % 8 == 0 ? linear % 8 * (blocks / 8) + linear / 8 : linear;
+  const int kvh = place / gridDim.x, worker = place % gridDim.x * WPB + (KW == 1 ? w : 0);
 
-  // request r has the tiles that begin at starts[r] * G / QT + r: intervals of slots that are always wide enough
-  int r = -1;
-  for (int i = 0; i < a.R; i += 64) {
-    bool before = false;
-    if (i + lane < a.R) before = (int64_t)((uint64_t)min(max(a.starts[i + lane], (int64_t)0), a.N) * a.G / QT) + i + lane <= slot;
-    r += __popcll(__ballot(before));
-  }
-  if (r < 0) return;
-  r = __builtin_amdgcn_readfirstlane(r);
-  const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), stop = min(max(a.starts[r + 1], start), a.N);
-  const int64_t tile = slot - (start * a.G / QT + r), columns = (stop - start) * a.G;
-  if (tile * QT >= columns) return;
-  if (a.which == 1 ? columns > 16 : a.which == 2 && columns <= 16) return;
-  const int64_t most = a.M << a.page_shift, said = a.lens[r], len = min(max(said, (int64_t)0), most), n = stop - start;
-  if (said > most && tile == 0 && blockIdx.z == 0 && kvh == 0 && threadIdx.x % (KW * 64) == 0) atomicAdd(a.errors, 1ull);
-
-  // this lane's columns: row of q and head, newest and oldest key they see
-  int64_t rows[NC];
-  int heads[NC];
-  int hi[NC], lo[NC];
-  bool live[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int64_t x = tile * QT + c * 16 + col;
-    live[c] = x < columns;
-    const int64_t i = live[c] ? x / a.G : 0;
-    rows[c] = start + i;
-    heads[c] = kvh * a.G + (live[c] ? (int)(x - i * a.G) : 0);
-    const int64_t p = said - n + i;
-    hi[c] = live[c] ? (int)min(max(p, (int64_t)-1), len - 1) : -1;
-    lo[c] = a.window > 0 ? (int)min(max(p - a.window + 1, (int64_t)0), len) : 0;
-  }
-  // of the tile's first and last token: every live column sees [lo_last, hi_first], none sees outside [lo_first, hi_last]
-  const int64_t p_first = said - n + tile * QT / a.G, p_last = said - n + (min((tile + 1) * QT, columns) - 1) / a.G;
-  const int hi_first = (int)min(max(p_first, (int64_t)-1), len - 1), hi_last = (int)min(max(p_last, (int64_t)-1), len - 1);
-  const int lo_first = a.window > 0 ? (int)min(max(p_first - a.window + 1, (int64_t)0), len) : 0, lo_last = a.window > 0 ? (int)min(max(p_last - a.window + 1, (int64_t)0), len) : 0;
-  const int step0 = lo_first / kStep, steps = max(hi_last / kStep + 1 - step0, 0) * (hi_last >= 0);
-  const int share = max((steps + a.splits - 1) / a.splits, a.least), parts = max((steps + share - 1) / share, 1);
-  const int z = blockIdx.z;
-  if (z >= parts) return;
-  const int s_begin = step0 + z * share, s_end = step0 + min(steps, (z + 1) * share);
-
-  kv_bf16x8 qf[NC][KS][TERMS];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const T *src = (const T *)a.q + rows[c] * a.q_row + (int64_t)heads[c] * a.q_head;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = TAIL && s == KS - 1 ? KN * 64 + 8 * g : (s / 2) * 64 + 16 * g + 8 * (s & 1);
-      float x[8];
-      if (a.q_aligned && d0 + 8 <= a.D) {
-        struct alignas(16) Eight { T v[8]; };
-        const Eight e = *reinterpret_cast<const Eight *>(src + d0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = live[c] ? (float)Scalar<T>::load(&e.v[j]) : 0.f;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = live[c] && d0 + j < a.D ? (float)Scalar<T>::load(src + d0 + j) : 0.f;
+  // ------------------------------------------------ this worker's first request and tile, and how far its share goes
+  // Every wave sums over the requests by itself, 64 at a time, without LDS or barriers: tiles, if each is a worker's, or their units.  (The code
+  // is kept short all through: a wave runs most of it once, at the rate at which instructions arrive.)
+  KvRequest req;
+  int r = -1, tile = 0;
+  int64_t from = 0, left = 1, share = 1, tile_at = 0;   // `from` units of the tile are others'; tile_at: units before the tile
+  {
+    KvRequest x;
+    int64_t own = 0, upto = 0, total = 0, u = worker;
+    for (int pass = 0; pass < 2 && r < 0; ++pass) {
+      int64_t at = 0;
+#pragma unroll 1
+      for (int i = 0; i < a.R; i += 64) {
+        if (pass == 0 || a.R > 64) {
+          x.tiles = 0;
+          if (i + lane < a.R) x = kv_request<QT>(a, i + lane);
+          own = a.workers == 0 ? x.tiles : x.tiles ? kv_units_before(a, x, x.tiles) : 0;
+          upto = at + wave_scan(own, lane);
+        }
+        const uint64_t here = __ballot(pass == 1 && u < upto);
+        if (here) {
+          const int f = __builtin_ctzll(here);
+          r = i + f;
+          tile_at = lane_of(upto - own, f);
+          req.start = __builtin_amdgcn_readlane(x.start, f);
+          req.n = __builtin_amdgcn_readlane(x.n, f);
+          req.len = __builtin_amdgcn_readlane(x.len, f);
+          req.first = __builtin_amdgcn_readlane(x.first, f);
+          req.tiles = __builtin_amdgcn_readlane(x.tiles, f);
+          break;
+        }
+        at = lane_of(upto, 63);
       }
-      union { kv_bf16x2 p[4]; kv_bf16x8 v; } u[TERMS];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        kv_bf16x2 t[TERMS];
-        kv_split2<TERMS>(x[2 * j], x[2 * j + 1], t);
-#pragma unroll
-        for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
+      if (pass == 0) {
+        total = at;
+        if (a.workers) {
+          share = max((int64_t)((double)total * a.per_worker) + 1, (int64_t)a.least * kUnits);   // times the workers: no less than the total
+          u = worker * share;
+          if ((KW == 1 ? lane : threadIdx.x) == 0) a.join[(int64_t)kvh * a.workers + worker].first = -1;
+        }
+        if (u >= total) return;
       }
-#pragma unroll
-      for (int i = 0; i < TERMS; ++i) qf[c][s][i] = u[i].v;
+    }
+    if (r < 0) return;
+    if (a.workers) {
+      int lo = 0, hi = req.tiles - 1;   // the tile that unit u lies in
+#pragma unroll 1
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (kv_units_before(a, req, mid) <= u - tile_at) lo = mid;
+        else hi = mid - 1;
+      }
+      tile = lo;
+      tile_at += kv_units_before(a, req, tile);
+      from = u - tile_at;
+      left = min(share, total - u);
+    } else {
+      tile = (int)(u - tile_at);
+      left = kv_units(a, req, tile);
     }
   }
 
-  const uint32_t *const table = a.tables + (int64_t)r * a.table_ld;
   const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
   const int slot_mask = (1 << a.page_shift) - 1, k_group = col >> 2;
-  // Of sixteen keys from `key` on: their page, and whether it is there.  Behind the context page 0 stands in.
-  struct Page { uint32_t id; bool there; };
-  auto page_of = [&](int key) __attribute__((always_inline)) {
-    const bool inside = key < len;
-    const uint32_t id = table[inside ? key >> a.page_shift : 0];
-    return Page{inside && id < a.pages ? id : 0u, inside && id < a.pages};
-  };
-  auto lost = [&](const Page &p, int key) __attribute__((always_inline)) { return key < len && !p.there; };
-
-  struct Keys { kv_u32x4 x[KN ? KN : 1][4]; kv_u32x2 tail[4]; };
-  struct Step { Keys k; float ks, vs; Page of_v; };
   // Features behind the cache's last are read again from its beginning: q is zero there.
   int k_at[KN ? KN : 1];
 #pragma unroll
   for (int i = 0; i < KN; ++i) k_at[i] = i * 64 + 16 * g < a.features ? i * 64 + 16 * g : 0;
   const int tail_at = KN * 64 + 8 * g < a.features ? KN * 64 + 8 * g : 0;
-  auto load_keys = [&](int st, Page pk, Page pv) __attribute__((always_inline)) {
-    Step s;
-    s.of_v = pv;
-    const int64_t ph = (int64_t)pv.id * a.Hkv + kvh;
-    s.ks = a.k_scale[ph];
-    s.vs = a.v_scale[ph];
-    const int key = st * kStep + 16 * k_group + (col & 3);
-    const uint8_t *base = a.k + ((int64_t)pk.id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * a.features;
+  int v_at[VT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < VT; ++t) v_at[t] = (16 * t + col < a.features ? 16 * t + col : 0) << a.page_shift;
+
+  bool first = true;   // of the worker's tiles
+  for (;; first = false) {
+    // ---------------------------------------------- the tile: its columns, the steps of it that are this worker's
+    const int64_t size = kv_units(a, req, tile), to = min(size, from + left);
+    const int len = req.len, columns = req.n * a.G;
+    int rows[NC], heads[NC], hi[NC], lo[NC];
+    bool live[NC];
+    // how far token i sees: keys lo .. hi
+    auto token = [&](int x) { return (int)(((double)x + 0.5) * a.per_group); };
+    auto newest = [&](int i) { return min(max(req.first + i, -1), len - 1); };
+    auto oldest = [&](int i) { return max(max(req.first + i, -1) - a.window + 1, 0); };
 #pragma unroll
-      for (int i = 0; i < KN; ++i) s.k.x[i][t] = *reinterpret_cast<const kv_u32x4 *>(base + 4 * t * a.features + k_at[i]);
-      if (TAIL) s.k.tail[t] = *reinterpret_cast<const kv_u32x2 *>(base + 4 * t * a.features + tail_at);
+    for (int c = 0; c < NC; ++c) {
+      const int x = tile * QT + c * 16 + col;
+      live[c] = x < columns;
+      const int i = live[c] ? token(x) : 0;   // (a column behind the last repeats the first, and goes nowhere)
+      rows[c] = req.start + i;
+      heads[c] = kvh * a.G + (live[c] ? x - i * a.G : 0);
+      hi[c] = live[c] ? newest(i) : -1;
+      lo[c] = oldest(i);
     }
-    return s;
-  };
+    // of the tile's first and last token: every live column sees lo_last .. hi_first, none sees outside lo_first .. hi_last
+    const int i_first = token(tile * QT), i_last = token(min((tile + 1) * QT, columns) - 1);
+    const int hi_first = newest(i_first), hi_last = newest(i_last), lo_first = oldest(i_first), lo_last = oldest(i_last);
+    const int step0 = lo_first / kStep, steps = hi_last >= lo_first ? hi_last / kStep + 1 - step0 : 0;
+    const int s_begin = step0 + (int)min((int64_t)steps, from / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, to / kUnits));
 
-  kv_f32x4 o[NC][VT];
-  float m[NC], l[NC];
+    kv_bf16x8 qf[NC][KS][TERMS];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m[c] = kNoScore;
-    l[c] = 0.f;
+    for (int c = 0; c < NC; ++c) {
+      const T *src = (const T *)a.q + (int64_t)rows[c] * a.q_row + (int64_t)heads[c] * a.q_head;
 #pragma unroll
-    for (int t = 0; t < VT; ++t) o[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  constexpr int STRIDE = KW;
-  int st = s_begin + (KW == 1 ? 0 : w);
-  bool missing = false;
-  if (st < s_end) {
-    const int last = s_end - 1;
-    Page pk = page_of(st * kStep + 16 * k_group), pv = page_of(st * kStep + 16 * g);
-    Step now = load_keys(st, pk, pv);
-    int ahead = min(st + STRIDE, last);
-    Page nk = page_of(ahead * kStep + 16 * k_group), nv = page_of(ahead * kStep + 16 * g);
-    for (; st < s_end; st += STRIDE) {
-      const int key0 = st * kStep + 16 * g;   // this lane group's first
-      kv_u32x4 v[VT];
-      {
-        const uint8_t *base = a.v + ((int64_t)now.of_v.id * a.Hkv + kvh) * head_bytes + (key0 & slot_mask);
-#pragma unroll
-        for (int t = 0; t < VT; ++t) {
-          const int d = 16 * t + col;
-          v[t] = *reinterpret_cast<const kv_u32x4 *>(base + ((int64_t)(d < a.features ? d : 0) << a.page_shift));
-        }
-      }
-      kv_f32x4 s[NC][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < KS; ++e) {
-          kv_bf16x8 f;
-          if (TAIL && e == KS - 1) f = kv_unpack<FMT>(now.k.tail[t].x, now.k.tail[t].y);
-          else f = kv_unpack<FMT>(now.k.x[e / 2][t][2 * (e & 1)], now.k.x[e / 2][t][2 * (e & 1) + 1]);
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < TERMS; ++i) s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[c][e][i], s[c][t], 0, 0, 0);
-        }
-      }
-      const Page of_v = now.of_v;
-      const float ks = of_v.there ? now.ks * a.scale_log2 : 0.f, vs = of_v.there ? now.vs : 0.f;
-      const int next = min(st + STRIDE, last);
-      now = load_keys(next, nk, nv);
-      ahead = min(next + STRIDE, last);
-      nk = page_of(ahead * kStep + 16 * k_group);
-      nv = page_of(ahead * kStep + 16 * g);
-
-      const bool gone = lost(of_v, key0);
-      missing |= gone;
-      const bool edge = (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone);
-      if ((st + 1) * kStep > len || __any(gone)) {
-        // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
-        const int valid = of_v.there ? (int)min(len - key0, (int64_t)16) : 0;
-        uint32_t keep[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int b = min(max(valid - 4 * j, 0), 4);
-          keep[j] = b == 4 ? 0xffffffffu : (1u << 8 * b) - 1;
-        }
-#pragma unroll
-        for (int t = 0; t < VT; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[t][j] &= keep[j];
-      }
-      kv_bf16x8 pf[NC][2][TERMS];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float top = kNoScore;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float x = s[c][t][j] * ks;
-            if (edge) {
-              const int key = key0 + 4 * t + j;
-              x = key <= hi[c] && key >= lo[c] && of_v.there ? x : -INFINITY;
-            }
-            s[c][t][j] = x;
-            top = fmaxf(top, x);
-          }
-        top = column_max(top);
-        // a maximum that grew by less than 2^8 waits: weights stay below 2^8, and sums in f32 lose nothing by it
-        if (__any(top > m[c] + 8.f)) {
-          const float up = fmaxf(m[c], top), f = __builtin_amdgcn_exp2f(m[c] - up);
-          m[c] = up;
-          l[c] *= f;
-#pragma unroll
-          for (int t = 0; t < VT; ++t) o[c][t] *= f;
-        }
-        float p[16];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = __builtin_amdgcn_exp2f(s[c][t][j] - m[c]);
-            l[c] += x;
-            p[4 * t + j] = x * vs;
-          }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          union { kv_bf16x2 p[4]; kv_bf16x8 v; } f[TERMS];
+      for (int s = 0; s < KS; ++s) {
+        const int d0 = TAIL && s == KS - 1 ? KN * 64 + 8 * g : (s / 2) * 64 + 16 * g + 8 * (s & 1);
+        struct alignas(16) Eight { T v[8]; } e = *reinterpret_cast<const Eight *>(src + (d0 < a.D ? d0 : 0));
+        if (d0 >= a.D) memset(&e, 0, sizeof(e));
+        if constexpr (TERMS == 1) {
+          qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, e);
+        } else {
+          union { kv_bf16x2 p[4]; kv_bf16x8 v; } u[TERMS];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             kv_bf16x2 t[TERMS];
-            kv_split2<TERMS>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], t);
+            kv_split2<TERMS>((float)Scalar<T>::load(&e.v[2 * j]), (float)Scalar<T>::load(&e.v[2 * j + 1]), t);
 #pragma unroll
-            for (int i = 0; i < TERMS; ++i) f[i].p[j] = t[i];
+            for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
           }
 #pragma unroll
-          for (int i = 0; i < TERMS; ++i) pf[c][u][i] = f[i].v;
+          for (int i = 0; i < TERMS; ++i) qf[c][s][i] = u[i].v;
         }
       }
+    }
+
+    // ---------------------------------------------- the cache
+    const uint32_t *const table = a.tables + (int64_t)r * a.table_ld;
+    // Of sixteen keys from `key` on: their page, and whether it is there.  Behind the context page 0 stands in.  An entry is asked for two
+    // steps ahead and looked at one step ahead: looked at sooner, it would wait for the loads that went out with it.
+    struct Page { uint32_t id; bool there; };
+    auto entry_of = [&](int key) __attribute__((always_inline)) { return table[key < len ? key >> a.page_shift : 0]; };
+    auto page_of = [&](uint32_t id, int key) __attribute__((always_inline)) {
+      const bool there = key < len && id < a.pages;
+      return Page{there ? id : 0u, there};
+    };
+    struct Step { kv_u32x4 k[KN ? KN : 1][4]; kv_u32x2 tail[4]; kv_u32x4 v[VT]; };
+    struct Scales { float k, v; bool there; };
+    Step now;
+    auto scales_of = [&](Page pv) __attribute__((always_inline)) {
+      const int64_t ph = (int64_t)pv.id * a.Hkv + kvh;
+      return Scales{a.k_scale[ph], a.v_scale[ph], pv.there};
+    };
+    auto load_keys = [&](int st, Page pk) __attribute__((always_inline)) {
+      Step &s = now;
+      const int key = st * kStep + 16 * k_group + (col & 3);
+      const uint8_t *base = a.k + ((int64_t)pk.id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * a.features;
 #pragma unroll
-      for (int t = 0; t < VT; ++t)
+      for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const kv_bf16x8 f = kv_unpack<FMT>(v[t][2 * u], v[t][2 * u + 1]);
+        for (int i = 0; i < KN; ++i) s.k[i][t] = fetch<KW != 1>(base + 4 * t * a.features + k_at[i]);
+        if (TAIL) s.tail[t] = *reinterpret_cast<const kv_u32x2 *>(base + 4 * t * a.features + tail_at);
+      }
+    };
+    auto load_values = [&](int st, Page pv) __attribute__((always_inline)) {
+      const uint8_t *values = a.v + ((int64_t)pv.id * a.Hkv + kvh) * head_bytes + ((st * kStep + 16 * g) & slot_mask);
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+      for (int t = 0; t < VT; ++t) now.v[t] = fetch<KW != 1>(values + v_at[t]);
+    };
+
+    kv_f32x4 o[NC][VT];
+    float m[NC], l[NC];
 #pragma unroll
-            for (int i = 0; i < TERMS; ++i) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], o[c][t], 0, 0, 0);
+    for (int c = 0; c < NC; ++c) {
+      m[c] = kNoScore;
+      l[c] = 0.f;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) o[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int st = s_begin + (KW == 1 ? 0 : w);
+    bool missing = false;
+    if (st < s_end) {
+      const int last = s_end - 1;
+      int next = min(st + KW, last);
+      uint32_t nk = entry_of(st * kStep + 16 * k_group), nv = entry_of(st * kStep + 16 * g);
+      Scales scales;
+      {
+        const Page pk = page_of(nk, st * kStep + 16 * k_group), pv = page_of(nv, st * kStep + 16 * g);
+        nk = entry_of(next * kStep + 16 * k_group);
+        nv = entry_of(next * kStep + 16 * g);
+        scales = scales_of(pv);
+        load_keys(st, pk);
+        load_values(st, pv);
+      }
+      for (; st < s_end; st += KW) {
+        const int ahead = min(next + KW, last);
+        const uint32_t ak = entry_of(ahead * kStep + 16 * k_group), av = entry_of(ahead * kStep + 16 * g);
+        const Page of_k = page_of(nk, next * kStep + 16 * k_group), of_v = page_of(nv, next * kStep + 16 * g);
+        const Scales coming = scales_of(of_v);   // (ahead of the keys: what a step hands to the next must not wait for those)
+        const int key0 = st * kStep + 16 * g;   // this lane group's first
+        const bool there = scales.there, gone = key0 < len && !there;
+        missing |= gone;
+        if ((st + 1) * kStep > len || __any(gone)) {
+          // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
+          const int valid = there ? (int)min(len - key0, (int64_t)16) : 0;
+          uint32_t keep[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int b = min(max(valid - 4 * j, 0), 4);
+            keep[j] = b == 4 ? 0xffffffffu : (1u << 8 * b) - 1;
+          }
+#pragma unroll
+          for (int t = 0; t < VT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) now.v[t][j] &= keep[j];
         }
-    }
-  }
-  if (__any(missing) && kvh == 0 && lane == 0) atomicAdd(a.errors, 1ull);
+        kv_f32x4 s[NC][4];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) l[c] = column_sum(l[c]);
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) s[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < KS; ++e) {
+            kv_bf16x8 f;
+            if (TAIL && e == KS - 1) f = kv_unpack<FMT>(now.tail[t].x, now.tail[t].y);
+            else f = kv_unpack<FMT>(now.k[e / 2][t][2 * (e & 1)], now.k[e / 2][t][2 * (e & 1) + 1]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[c][e][i], s[c][t], 0, 0, 0);
+          }
+        }
+        // With several tiles to share them V's fragments are made here, beside the scores' products, and its registers are free for the next step's
+        kv_bf16x8 vf[HOIST ? VT : 1][2];
+        if constexpr (HOIST) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) vf[t][u] = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
+        }
+        const float ks = scales.k * a.scale_log2, vs = there && scales.v > 0.f ? scales.v : 1.f;
+        load_keys(next, of_k);
+        if constexpr (HOIST) load_values(next, of_v);
 
-  if constexpr (KW > 1) {
-    // the upper half of the waves hands its sums to the lower, until one is left; values lie in LDS as in registers
-    static_assert(NC == 1, "waves that share steps have one tile of 16 columns");
-    __shared__ kv_f32x4 sums[KW / 2][VT][64];
-    __shared__ float stats[KW / 2][2][64];
+        // log2(vs): its exponent, to which the logarithm of a power of two adds nothing
+        const uint32_t bits = __float_as_uint(vs);
+        const float up_v = (float)((int)(bits >> 23) - 127) + __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)), over_v = __builtin_amdgcn_rcpf(vs);
+        const bool edge = (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone);
+        const float times = edge ? 1.f : ks;
+        float top[NC];
+        bool grows = false;
 #pragma unroll
-    for (int half = KW / 2; half > 0; half /= 2) {
-      if (w >= half && w < 2 * half) {
+        for (int c = 0; c < NC; ++c) {
+          if (edge)
 #pragma unroll
-        for (int t = 0; t < VT; ++t) sums[w - half][t][lane] = o[0][t];
-        stats[w - half][0][lane] = m[0];
-        stats[w - half][1][lane] = l[0];
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int key = key0 + 4 * t + j;
+                s[c][t][j] = key <= hi[c] && key >= lo[c] && there ? s[c][t][j] * ks : -INFINITY;
+              }
+          float most = s[c][0][0], least = s[c][0][0];
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, s[c][t][j]), least = fminf(least, s[c][t][j]);
+          top[c] = column_max(fmaxf(times < 0.f ? least * times : most * times, kNoScore));
+          grows |= top[c] > m[c] + 8.f;
+        }
+        // a maximum that grew by less than 2^8 waits: weights stay below 2^8, and sums in f32 lose nothing by it
+        if (__any(grows)) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const float up = fmaxf(m[c], top[c]), f = __builtin_amdgcn_exp2f(m[c] - up);
+            m[c] = up;
+            l[c] *= f;
+#pragma unroll
+            for (int t = 0; t < VT; ++t) o[c][t] *= f;
+          }
+        }
+        kv_bf16x8 pf[NC][2][TERMS];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float down = up_v - m[c];
+          float p[16], sum = 0.f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(s[c][t][j], times, down));
+              sum += p[4 * t + j];
+            }
+          l[c] = fmaf(sum, over_v, l[c]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            union { kv_bf16x2 p[4]; kv_bf16x8 v; } f[TERMS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              kv_bf16x2 t[TERMS];
+              kv_split2<TERMS>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], t);
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) f[i].p[j] = t[i];
+            }
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) pf[c][u][i] = f[i].v;
+          }
+          if constexpr (HOIST)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int t = 0; t < VT; ++t)
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t][u], pf[c][u][i], o[c][t], 0, 0, 0);
+        }
+        if constexpr (!HOIST) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const kv_bf16x8 f = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], o[c][t], 0, 0, 0);
+            }
+          load_values(next, of_v);
+        }
+        next = ahead;
+        nk = ak;
+        nv = av;
+        scales = coming;
       }
-      __syncthreads();
-      if (w < half) {
-        const float m2 = stats[w][0][lane], l2 = stats[w][1][lane], up = fmaxf(m[0], m2);
-        const float f1 = __builtin_amdgcn_exp2f(m[0] - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
-        m[0] = up;
-        l[0] = l[0] * f1 + l2 * f2;
-#pragma unroll
-        for (int t = 0; t < VT; ++t) o[0][t] = o[0][t] * f1 + sums[w][t][lane] * f2;
-      }
-      __syncthreads();
     }
-    if (w > 0) return;
-  }
+    if (kvh == 0) {
+      const bool past = from == 0 && tile == 0 && (KW == 1 || w == 0) && a.lens[r] > a.M << a.page_shift;
+      if ((__any(missing) || past) && lane == 0) atomicAdd(a.errors, 1ull);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) l[c] = column_sum(l[c]);
 
+    if constexpr (KW > 1) {
+      // the upper half of the waves hands its sums to the lower, until one is left; values lie in LDS as in registers
+      static_assert(NC == 1, "waves that share steps have one tile of 16 columns");
+      __shared__ kv_f32x4 sums[KW / 2][VT][64];
+      __shared__ float stats[KW / 2][2][64];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (!live[c]) continue;
-    const int64_t at = rows[c] * a.Hq + heads[c];
-    if (parts > 1) {
-      const int64_t e = at * a.splits + z;
-      if (g == 0) {
-        a.part_m[e] = m[c];
-        a.part_l[e] = l[c];
-        if (z == 0) a.parts[at] = parts;
+      for (int half = KW / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (w >= half && w < 2 * half) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t) sums[w - half][t][lane] = o[0][t];
+          stats[w - half][0][lane] = m[0];
+          stats[w - half][1][lane] = l[0];
+        }
+        __syncthreads();
+        if (w < half) {
+          const float m2 = stats[w][0][lane], l2 = stats[w][1][lane], up = fmaxf(m[0], m2);
+          const float f1 = __builtin_amdgcn_exp2f(m[0] - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
+          m[0] = up;
+          l[0] = l[0] * f1 + l2 * f2;
+#pragma unroll
+          for (int t = 0; t < VT; ++t) o[0][t] = o[0][t] * f1 + sums[w][t][lane] * f2;
+        }
       }
-#pragma unroll
-      for (int t = 0; t < VT; ++t)
-        if (16 * t < a.features) *reinterpret_cast<kv_f32x4 *>(a.part + e * a.features + 16 * t + 4 * g) = o[c][t];
-      continue;
     }
-    if (a.splits > 1 && g == 0) a.parts[at] = 1;
-    const float f = l[c] == 0.f ? 0.f : 1.f / l[c];
-    T *dst = (T *)a.out + at * a.D;
+
+    // ---------------------------------------------- out, or to the tile's other parts
+    const bool whole = from == 0 && to == size;
+    if (KW == 1 || w == 0) {
+      const int64_t own = (int64_t)kvh * a.workers + worker, part = (2 * own + !first) * QT;
 #pragma unroll
-    for (int t = 0; t < VT; ++t) {
-      const int d = 16 * t + 4 * g;
-      struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
+      for (int c = 0; c < NC; ++c) {
+        if (!live[c]) continue;
+        if (!whole) {
+          const int64_t e = part + c * 16 + col;
+          if (g == 0) {
+            a.part_m[e] = m[c];
+            a.part_l[e] = l[c];
+          }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], l[c] == 0.f ? 0.f : o[c][t][j] * f);
-      if (a.out_aligned && d + 4 <= a.D) *reinterpret_cast<Four *>(dst + d) = y;
-      else
+          for (int t = 0; t < VT; ++t)
+            if (16 * t < a.features) *reinterpret_cast<kv_f32x4 *>(a.part + e * a.features + 16 * t + 4 * g) = o[c][t];
+          continue;
+        }
+        const float f = l[c] == 0.f ? 0.f : 1.f / l[c];
+        T *dst = (T *)a.out + ((int64_t)rows[c] * a.Hq + heads[c]) * a.D + 4 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d + j < a.D) dst[d + j] = y.v[j];
+        for (int t = 0; t < VT; ++t) {
+          struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], l[c] == 0.f ? 0.f : o[c][t][j] * f);
+          if (16 * t + 4 * g < a.D) *reinterpret_cast<Four *>(dst + 16 * t) = y;
+        }
+      }
+      if (!whole && to == size && lane == 0) {
+        int64_t begin = (int64_t)((double)tile_at / (double)share);
+        begin += begin * share > tile_at ? -1 : (begin + 1) * share <= tile_at ? 1 : 0;
+        a.join[own] = KvJoin{(int)begin, tile_at != begin * share, req.start, tile * QT, min(QT, columns - tile * QT)};
+      }
+    }
+    left -= to - from;
+    if (a.workers == 0 || left <= 0) return;
+    from = 0;
+    tile_at += size;
+    if (++tile >= req.tiles) {
+      tile = 0;
+      do {
+        if (++r >= a.R) return;
+        req = kv_request<QT>(a, r);
+      } while (req.tiles == 0);
     }
   }
 }
 
-// The parts of a row and head to its output: a wave each.
-template <typename T> __global__ void __launch_bounds__(256) k_kv_attention_merge(KvAttnArgs a, int64_t begin, int64_t end) {
-  const int64_t at = begin + (int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (at >= end) return;
-  // rows that belong to no request have no parts
-  const int64_t row = at / a.Hq;
-  if (row < min(max(a.starts[0], (int64_t)0), a.N) || row >= min(max(a.starts[a.R], (int64_t)0), a.N)) return;
-  const int parts = min(a.parts[at], a.splits);
-  if (parts <= 1) return;
-  float m = kNoScore;
-  for (int z = 0; z < parts; ++z) m = fmaxf(m, a.part_m[at * a.splits + z]);
-  float l = 0.f, o[kKvMaxFeatures / 64] = {};
-  for (int z = 0; z < parts; ++z) {
-    const int64_t e = at * a.splits + z;
-    const float f = __builtin_amdgcn_exp2f(a.part_m[e] - m);
-    l = fmaf(a.part_l[e], f, l);
+// The parts of tiles that workers share, to the output: a block for each worker that had a tile's last part.
+template <typename T> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, int QT) {
+  const int64_t worker = blockIdx.x, own = (int64_t)blockIdx.y * a.workers + worker;
+  const KvJoin j = a.join[own];
+  if (j.first < 0) return;
+  const int F4 = a.features / 4;
+  for (int e = threadIdx.x; e < j.columns * F4; e += 256) {
+    const int c = e / F4, d = (e - c * F4) * 4, x = j.column + c, i = x / a.G;
+    auto part_of = [&](int64_t k) { return (2 * ((int64_t)blockIdx.y * a.workers + k) + (k == j.first ? j.place : 0)) * QT + c; };
+    float m = kNoScore, l = 0.f;
+    kv_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t k = j.first; k <= worker; k += 4) {   // four parts asked for at a time
+      float pm[4], pl[4], up = m;
+      kv_f32x4 y[4];
 #pragma unroll
-    for (int i = 0; i < kKvMaxFeatures / 64; ++i)
-      if (i * 64 + lane < a.features) o[i] = fmaf(a.part[e * a.features + i * 64 + lane], f, o[i]);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t p = part_of(min(k + u, worker));
+        pm[u] = a.part_m[p];
+        pl[u] = a.part_l[p];
+        y[u] = *reinterpret_cast<const kv_f32x4 *>(a.part + p * a.features + d);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (k + u > worker) pm[u] = kNoScore, pl[u] = 0.f, y[u] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+        up = fmaxf(up, pm[u]);
+      }
+      const float f = __builtin_amdgcn_exp2f(m - up);
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float g = __builtin_amdgcn_exp2f(pm[u] - up);
+        l = fmaf(pl[u], g, l);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[v] = fmaf(y[u][v], g, o[v]);
+      }
+      m = up;
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + (((int64_t)j.start + i) * a.Hq + (int64_t)blockIdx.y * a.G + x - i * a.G) * a.D + d;
+    struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) Scalar<T>::store(&y.v[u], l == 0.f ? 0.f : o[u] * f);
+    if (d < a.D) *reinterpret_cast<Four *>(dst) = y;
   }
-  const float f = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int i = 0; i < kKvMaxFeatures / 64; ++i)
-    if (i * 64 + lane < a.D) Scalar<T>::store((T *)a.out + at * a.D + i * 64 + lane, l == 0.f ? 0.f : o[i] * f);
 }
 
-template <typename T, int FMT, int VT, int NC, int KW> static void launch_tiles(hipStream_t st, const KvAttnArgs &a) {
-  const int64_t slots = a.N * a.G / (16 * NC) + a.R;
-  hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, NC, KW>), dim3((unsigned)(KW == 1 ? (slots + 3) / 4 : slots), (unsigned)a.Hkv, (unsigned)a.splits), dim3(256), 0, st, a);
-}
-
-// Tiles of 16 columns to a wave that has a tile to itself: as many as registers hold.
+// Tiles of 16 columns to a wave that is a worker by itself: as many as registers hold.
 template <typename T> constexpr int wide_tiles(int features) { return (features <= 128 ? 2 : 1) * (KvTerms<T>::n == 1 ? 2 : 1); }
 
-template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, bool wide) {
-  constexpr int NC = wide_tiles<T>(16 * VT);
-  if (wide) {
-    a.which = 2;
-    launch_tiles<T, FMT, VT, NC, 1>(st, a);
-    RAI_TRY(launch_check("kv_attention"));
-    a.which = 1;
+// Rows of D features off 16-byte boundaries to ones of F, zeros behind the D; and the other way, of the rows that are a request's.
+struct KvRowsArgs {
+  const void *src;
+  void *dst;
+  int64_t row, head, N;          // strides of the rows that are not contiguous
+  int H, D, F, R;
+  const int64_t *starts;
+};
+template <typename T> __global__ void __launch_bounds__(256) k_kv_rows_widen(KvRowsArgs a) {
+  const int64_t total = a.N * a.H * a.F;
+  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+    const int64_t rh = e / a.F, n = rh / a.H;
+    const int d = (int)(e - rh * a.F), h = (int)(rh - n * a.H);
+    T v;
+    memset(&v, 0, sizeof(T));
+    if (d < a.D) v = ((const T *)a.src)[n * a.row + h * a.head + d];
+    ((T *)a.dst)[e] = v;
   }
-  launch_tiles<T, FMT, VT, 1, 4>(st, a);
+}
+template <typename T> __global__ void __launch_bounds__(256) k_kv_rows_narrow(KvRowsArgs a) {
+  const int64_t total = a.N * a.H * a.D, first = a.starts[0], last = a.starts[a.R];
+  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+    const int64_t rh = e / a.D, n = rh / a.H;
+    if (n >= first && n < last) ((T *)a.dst)[e] = ((const T *)a.src)[rh * a.F + e - rh * a.D];
+  }
+}
+
+// What a launch takes of the scratch: parts of tiles, and the words about them.
+struct KvPlanOfWork {
+  int workers, columns;          // of a key head; of a tile
+  size_t bytes(const KvAttnArgs &a) const { return workers ? (size_t)a.Hkv * workers * (2ll * columns * (a.features + 2) * 4 + sizeof(KvJoin)) : 0; }
+};
+template <typename T, int VT, int NC, int KW> static KvPlanOfWork plan_of_work(const KvAttnArgs &a, int64_t steps) {
+  constexpr int WPB = 4 / KW;
+  if (steps <= kv_alone(KW)) return {0, 16 * NC};
+  const int64_t workers = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC) * WPB / a.Hkv;
+  return {(int)(workers < WPB ? WPB : workers / WPB * WPB), 16 * NC};
+}
+
+template <typename T, int FMT, int VT, int NC, int KW> static int launch_tiles(hipStream_t st, KvAttnArgs a, int64_t steps, void *ws) {
+  constexpr int QT = 16 * NC, WPB = 4 / KW;
+  const KvPlanOfWork p = plan_of_work<T, VT, NC, KW>(a, steps);
+  a.each = (16 * QT + a.G - 1) / a.G;
+  a.workers = p.workers;
+  if (a.workers) {
+    const int64_t parts = 2 * QT * (int64_t)a.Hkv * a.workers;
+    a.least = kv_least(KW);
+    a.per_worker = 1.0 / a.workers;
+    a.part = (float *)ws;
+    a.part_m = a.part + parts * a.features;
+    a.part_l = a.part_m + parts;
+    a.join = (KvJoin *)(a.part_l + parts);
+  }
+  const int64_t slots = a.which == 1 ? a.R : a.N * a.G / QT + a.R, x = a.workers ? a.workers / WPB : (slots + WPB - 1) / WPB;
+  hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, NC, KW>), dim3((unsigned)x, (unsigned)a.Hkv), dim3(256), 0, st, a);
   RAI_TRY(launch_check("kv_attention"));
-  if (a.splits > 1) {
-    const int64_t waves = a.N * a.Hq;
-    dim3 grid;
-    RAI_TRY(grid_of_blocks((waves + 3) / 4, 256, &grid));
-    hipLaunchKernelGGL((k_kv_attention_merge<T>), grid, dim3(256), 0, st, a, (int64_t)0, waves);
-    RAI_TRY(launch_check("kv_attention_merge"));
+  if (a.workers) {
+    hipLaunchKernelGGL((k_kv_attention_join<T>), dim3((unsigned)a.workers, (unsigned)a.Hkv), dim3(256), 0, st, a, QT);
+    RAI_TRY(launch_check("kv_attention_join"));
   }
   return RAI_OK;
 }
 
-template <typename T, int FMT> static int launch_by_features(hipStream_t st, const KvAttnArgs &a, bool wide) {
-  if (a.features <= 64) return launch_kv_attention<T, FMT, 4>(st, a, wide);
-  if (a.features <= 80) return launch_kv_attention<T, FMT, 5>(st, a, wide);
-  if (a.features <= 128) return launch_kv_attention<T, FMT, 8>(st, a, wide);
-  return launch_kv_attention<T, FMT, 16>(st, a, wide);
+template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, const KvRowsArgs &odd, bool wide, int64_t steps) {
+  constexpr int NC = wide_tiles<T>(16 * VT);
+  // the two launches run one after the other and may use the same scratch
+  size_t parts = plan_of_work<T, VT, 1, 4>(a, steps).bytes(a);
+  if (wide) {
+    const size_t others = plan_of_work<T, VT, NC, 1>(a, steps).bytes(a);
+    if (others > parts) parts = others;
+  }
+  const size_t rows = odd.src ? ((size_t)a.N * a.Hq * a.features * sizeof(T) + 15) / 16 * 16 : 0;
+  WorkspaceHold hold;
+  void *ws = nullptr;
+  if (parts + rows) RAI_TRY(workspace(a.dev, parts + 2 * rows, &ws, &hold));
+  const int64_t most = kNumCU * 32;
+  KvRowsArgs in = odd, back = odd;
+  if (odd.src) {
+    a.q = in.dst = (char *)ws + parts;
+    a.out = (char *)ws + parts + rows;
+    back.src = a.out;
+    a.q_row = (int64_t)a.Hq * a.features;
+    a.q_head = a.D = a.features;
+    const int64_t blocks = (a.N * a.Hq * a.features + 255) / 256;
+    hipLaunchKernelGGL((k_kv_rows_widen<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, in);
+    RAI_TRY(launch_check("kv_rows_widen"));
+  }
+  if (wide) {
+    a.which = 2;
+    RAI_TRY((launch_tiles<T, FMT, VT, NC, 1>(st, a, steps, ws)));
+    a.which = 1;
+  }
+  RAI_TRY((launch_tiles<T, FMT, VT, 1, 4>(st, a, steps, ws)));
+  if (odd.src) {
+    const int64_t blocks = (a.N * a.Hq * odd.D + 255) / 256;
+    hipLaunchKernelGGL((k_kv_rows_narrow<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, back);
+    RAI_TRY(launch_check("kv_rows_narrow"));
+  }
+  return RAI_OK;
+}
+
+template <typename T, int FMT> static int launch_by_features(hipStream_t st, const KvAttnArgs &a, const KvRowsArgs &odd, bool wide, int64_t steps) {
+  if (a.features <= 64) return launch_kv_attention<T, FMT, 4>(st, a, odd, wide, steps);
+  if (a.features <= 80) return launch_kv_attention<T, FMT, 5>(st, a, odd, wide, steps);
+  if (a.features <= 128) return launch_kv_attention<T, FMT, 8>(st, a, odd, wide, steps);
+  return launch_kv_attention<T, FMT, 16>(st, a, odd, wide, steps);
 }
 
 }  // namespace rai
@@ -521,32 +781,29 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
   a.k = c.k; a.v = c.v; a.k_scale = c.k_scale; a.v_scale = c.v_scale;
   a.pages = M == 0 ? 0 : c.pages;
   a.R = (int)R; a.Hq = (int)Hq; a.Hkv = c.heads; a.G = (int)(Hq / c.heads); a.D = (int)D;
-  a.features = c.features; a.page_shift = c.page_shift; a.window = window;
-  a.q_aligned = (uintptr_t)a.q % 16 == 0 && (N == 1 || a.q_row * es % 16 == 0) && (Hq == 1 || a.q_head * es % 16 == 0);
-  a.out_aligned = (uintptr_t)a.out % (4 * es) == 0 && D % 4 == 0;
+  a.features = c.features; a.page_shift = c.page_shift;
+  a.window = window > 0 ? window : INT32_MAX;
+  a.reach = window > 0 && window < INT32_MAX - kStep ? window + kStep : INT32_MAX;
+  a.per_group = 1.0 / a.G;
+  // rows off 16-byte boundaries, and heads of features in no whole eights, go through rows of the cache's features
+  const bool even = D % 8 == 0 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 16 == 0 && (N == 1 || a.q_row * es % 16 == 0) && (Hq == 1 || a.q_head * es % 16 == 0);
+  KvRowsArgs odd;
+  memset(&odd, 0, sizeof(odd));
+  if (!even) {
+    odd.src = a.q;
+    odd.dst = a.out;
+    odd.row = a.q_row;
+    odd.head = a.q_head;
+    odd.N = N; odd.H = a.Hq; odd.D = a.D; odd.F = a.features; odd.R = a.R;
+    odd.starts = a.starts;
+  }
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.errors = index_error_counter(dev);
 
+  a.dev = dev;
   const bool wide = N * a.G > 16 * R;   // some request has more than one tile of 16 columns
-  const int nc = q->dtype == RAI_BF16 ? wide_tiles<bf16_raw>(a.features) : wide_tiles<float>(a.features);
-  const int64_t tiles = (N * a.G / (wide ? 16 * nc : 16) + R) * a.Hkv, steps = (M * c.page + kStep - 1) / kStep;
-  int64_t splits = 2048 / tiles;
-  a.least = 8;
-  if (splits > (steps + a.least - 1) / a.least) splits = (steps + a.least - 1) / a.least;
-  if (splits > 64) splits = 64;
-  if (splits < 1) splits = 1;
-  a.splits = (int)splits;
-  WorkspaceHold hold;
-  if (splits > 1) {
-    const int64_t cells = N * Hq * splits;
-    void *ws = nullptr;
-    RAI_TRY(workspace(dev, (size_t)(cells * (a.features + 2) + N * Hq) * 4, &ws, &hold));
-    a.part = (float *)ws;
-    a.part_m = a.part + cells * a.features;
-    a.part_l = a.part_m + cells;
-    a.parts = (int *)(a.part_l + cells);
-  }
-#define KV_ATTENTION(T) return format == RAI_KV_E4M3 ? launch_by_features<T, RAI_KV_E4M3>(st, a, wide) : launch_by_features<T, RAI_KV_INT8>(st, a, wide)
+  const int64_t steps = (M * c.page + kStep - 1) / kStep;
+#define KV_ATTENTION(T) return format == RAI_KV_E4M3 ? launch_by_features<T, RAI_KV_E4M3>(st, a, odd, wide, steps) : launch_by_features<T, RAI_KV_INT8>(st, a, odd, wide, steps)
   if (q->dtype == RAI_BF16) KV_ATTENTION(bf16_raw);
   if (q->dtype == RAI_F16) KV_ATTENTION(f16_raw);
   KV_ATTENTION(float);
