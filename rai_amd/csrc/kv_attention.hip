@@ -22,11 +22,12 @@ struct KvAttnArgs {
   const float *k_scale, *v_scale;
   int64_t pages;
   int dev, R, Hq, Hkv, G, D, features, page_shift, window;
-  float scale_log2;              // scale * log2(e)
+  float scale_log2;              // |scale| * log2(e)
+  uint32_t turn;                 // the signs of two bf16 where the scale is negative
   double per_group;              // 1 / G
   int reach;                     // keys that the oldest token of a tile sees, at most
   int which;                     // requests served: 0 all, 1 those of up to 16 columns, 2 the others
-  int each;                      // sixteenths of a key that a tile sees more than the one before it
+  int each, extra;               // sixteenths of a key that a tile sees more than the one before it, and that its beginning and end are worth
   double per_worker;             // 1 / workers
   int workers;                   // of a key head, each with an even share of the steps; 0: a worker to a tile
   int least;                     // steps of a share at least
@@ -62,11 +63,8 @@ template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, u
   return u.v;
 }
 
-// ONCE: read by one tile alone, so not to be kept in the L2.
-template <bool ONCE> __device__ __forceinline__ kv_u32x4 fetch(const uint8_t *p) {
-  const kv_u32x4 *q = reinterpret_cast<const kv_u32x4 *>(p);
-  return ONCE ? __builtin_nontemporal_load(q) : *q;
-}
+// Read by one tile alone, so not to be kept in the L2.
+__device__ __forceinline__ kv_u32x4 fetch_once(const uint8_t *p) { return __builtin_nontemporal_load(reinterpret_cast<const kv_u32x4 *>(p)); }
 
 // How many bf16 hold a value of type T: products with codes are then exact, so f16 and f32 rows lose nothing on the bf16 matrix instructions.
 template <typename T> struct KvTerms;
@@ -106,22 +104,25 @@ constexpr float kNoScore = -3.402823466e38f;   // a running maximum before the f
 constexpr int kStep = 64;                      // keys of a step
 
 // Blocks of a kernel that a CU holds.
-constexpr int kv_blocks(int vt, int nc) { return nc > 1 || vt > 8 ? 1 : vt > 5 ? 2 : 3; }
-// Contexts of up to so many steps are not shared between workers.
-constexpr int kv_alone(int kw) { return kw == 1 ? 8 : 16; }
-constexpr int kv_least(int kw) { return kw == 1 ? 2 : 8; }
+constexpr int kv_blocks(int vt, int nc, int terms) { return vt > 8 || (nc > 1 && terms > 1 && vt > 4) ? 1 : nc > 1 || vt > 5 || terms > 1 ? 2 : 3; }
+// Contexts of up to so many steps are not shared between workers; of longer ones a worker has so many at least.
+constexpr int kv_alone(int nc) { return nc ? 8 : 16; }
+constexpr int kv_least(int nc) { return nc ? 2 : 8; }
+// Steps that a tile's beginning and end take as long as.
+constexpr int kv_extra(int nc) { return nc ? 2 : 8; }
 
 // How the work of a key head is dealt out.  A tile of a request is as long as the keys that its last row sees, which grows evenly from tile to
-// tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1).
+// tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1), and `extra` for its beginning and end
+// (queries, first loads, the merge), which a worker that goes on to another tile pays again.
 constexpr int kUnits = 16 * kStep;   // of a step
 struct KvRequest {
   int start, n, tiles;           // first row, new tokens
   int len, first;                // length, cut to its table's; position of the first new token
 };
 __device__ __forceinline__ int64_t kv_base(const KvAttnArgs &a, const KvRequest &q) { return 16ll * min(max(q.len - q.n, 0), a.reach); }
-__device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return kv_base(a, q) + (int64_t)a.each * (tile + 1); }
+__device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return kv_base(a, q) + a.extra + (int64_t)a.each * (tile + 1); }
 // of the tiles before `tile`
-__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return tile * kv_base(a, q) + a.each * (tile * (tile + 1) / 2); }
+__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return tile * (kv_base(a, q) + a.extra) + a.each * (tile * (tile + 1) / 2); }
 
 template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, int r) {
   KvRequest q;
@@ -146,90 +147,317 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 
-// The columns of a request and key head are its new tokens times the query heads of the group, G to a token; a tile is 16 NC of them.  A
-// step is 64 keys:
+// A worker's place in the work of a key head: its request and tile, and how far its share goes.
+struct KvWork {
+  KvRequest req;
+  int r, tile;
+  int64_t from, left;            // `from` units of the tile are others'
+  int64_t share, tile_at;        // units before the tile
+};
+// Every wave sums over the requests by itself, 64 at a time, without LDS or barriers: tiles, if each is a worker's, or their units.  (The code
+// around the steps is kept short all through: a wave runs it once, at the rate at which instructions arrive.)
+template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, int kvh, int worker, KvWork *out) {
+  const int lane = threadIdx.x & 63;
+  KvRequest x;
+  out->r = -1;
+  out->tile = 0;
+  out->from = 0;
+  out->left = out->share = 1;
+  int64_t own = 0, upto = 0, total = 0, u = worker;
+  for (int pass = 0; pass < 2 && out->r < 0; ++pass) {
+    int64_t at = 0;
+#pragma unroll 1
+    for (int i = 0; i < a.R; i += 64) {
+      if (pass == 0 || a.R > 64) {
+        x.tiles = 0;
+        if (i + lane < a.R) x = kv_request<QT>(a, i + lane);
+        own = a.workers == 0 ? x.tiles : x.tiles ? kv_units_before(a, x, x.tiles) : 0;
+        upto = at + wave_scan(own, lane);
+      }
+      const uint64_t here = __ballot(pass == 1 && u < upto);
+      if (here) {
+        const int f = __builtin_ctzll(here);
+        out->r = i + f;
+        out->tile_at = lane_of(upto - own, f);
+        out->req.start = __builtin_amdgcn_readlane(x.start, f);
+        out->req.n = __builtin_amdgcn_readlane(x.n, f);
+        out->req.len = __builtin_amdgcn_readlane(x.len, f);
+        out->req.first = __builtin_amdgcn_readlane(x.first, f);
+        out->req.tiles = __builtin_amdgcn_readlane(x.tiles, f);
+        break;
+      }
+      at = lane_of(upto, 63);
+    }
+    if (pass == 0) {
+      total = at;
+      if (a.workers) {
+        out->share = max((int64_t)((double)total * a.per_worker) + 1, (int64_t)a.least * kUnits);   // times the workers: no less than the total
+        u = worker * out->share;
+        if (threadIdx.x == 0) a.join[(int64_t)kvh * a.workers + worker].first = -1;
+      }
+      if (u >= total) return false;
+    }
+  }
+  if (out->r < 0) return false;
+  if (a.workers) {
+    int lo = 0, hi = out->req.tiles - 1;   // the tile that unit u lies in
+#pragma unroll 1
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (kv_units_before(a, out->req, mid) <= u - out->tile_at) lo = mid;
+      else hi = mid - 1;
+    }
+    out->tile = lo;
+    out->tile_at += kv_units_before(a, out->req, lo);
+    out->from = u - out->tile_at;
+    out->left = min(out->share, total - u);
+  } else {
+    out->tile = (int)(u - out->tile_at);
+    out->left = kv_units(a, out->req, out->tile);
+  }
+  return true;
+}
+// On to the next tile; false behind the worker's last.
+template <int QT> __device__ __forceinline__ bool kv_next(const KvAttnArgs &a, int64_t size, int64_t to, KvWork *k) {
+  k->left -= to - k->from;
+  if (a.workers == 0 || k->left <= 0) return false;
+  k->from = 0;
+  k->tile_at += size;
+  if (++k->tile >= k->req.tiles) {
+    k->tile = 0;
+    do {
+      if (++k->r >= a.R) return false;
+      k->req = kv_request<QT>(a, k->r);
+    } while (k->req.tiles == 0);
+  }
+  return true;
+}
+// The first part of a tile that others finish, or end, is said to the launch that joins them.
+template <int QT> __device__ __forceinline__ void kv_say_join(const KvAttnArgs &a, const KvWork &k, int64_t own, int columns) {
+  int64_t begin = (int64_t)((double)k.tile_at / (double)k.share);
+  begin += begin * k.share > k.tile_at ? -1 : (begin + 1) * k.share <= k.tile_at ? 1 : 0;
+  a.join[own] = KvJoin{(int)begin, k.tile_at != begin * k.share, k.req.start, k.tile * QT, min(QT, columns - k.tile * QT)};
+}
+
+// Which keys the tokens of a request see: of token i, oldest(i) .. newest(i).
+struct KvSeen {
+  int first, len, window;
+  double per_group;
+  __device__ __forceinline__ int token(int x) const { return (int)(((double)x + 0.5) * per_group); }   // of column x
+  __device__ __forceinline__ int newest(int i) const { return min(max(first + i, -1), len - 1); }
+  __device__ __forceinline__ int oldest(int i) const { return max(max(first + i, -1) - window + 1, 0); }
+};
+// Columns of a tile, 16 to a lane group's place in NC: row of q and head, and what they see.
+template <int NC> struct KvColumns {
+  int rows[NC], heads[NC], hi[NC], lo[NC];
+  bool live[NC];
+};
+template <int NC> __device__ __forceinline__ KvColumns<NC> kv_columns(const KvAttnArgs &a, const KvRequest &req, const KvSeen &see, int kvh, int x0, int columns) {
+  KvColumns<NC> k;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int x = x0 + c * 16 + (threadIdx.x & 15);
+    k.live[c] = x < columns;
+    const int i = k.live[c] ? see.token(x) : 0;   // (a column behind the last repeats the first, and goes nowhere)
+    k.rows[c] = req.start + i;
+    k.heads[c] = kvh * a.G + (k.live[c] ? x - i * a.G : 0);
+    k.hi[c] = k.live[c] ? see.newest(i) : -1;
+    k.lo[c] = see.oldest(i);
+  }
+  return k;
+}
+
+// How a key's F features go into products of 32: in pieces of 64, 16 neighbouring ones to a lane group, so that a lane's 16 bytes of codes serve two
+// products; what is left over by 8 bytes a lane where that is 32 or less.
+template <int VT> struct KvFeatures {
+  static constexpr int KR = VT % 4, KN = VT / 4 + (KR == 3), KS = 2 * KN + (KR == 1 || KR == 2);
+  static constexpr bool TAIL = KR == 1 || KR == 2;
+  static __device__ __forceinline__ int of_product(int s, int g) { return TAIL && s == KS - 1 ? KN * 64 + 8 * g : (s / 2) * 64 + 16 * g + 8 * (s & 1); }
+};
+template <typename T, int VT, int NC>
+__device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<NC> &k, kv_bf16x8 (&qf)[NC][KvFeatures<VT>::KS][KvTerms<T>::n]) {
+  constexpr int TERMS = KvTerms<T>::n;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const T *src = (const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head;
+#pragma unroll
+    for (int s = 0; s < KvFeatures<VT>::KS; ++s) {
+      const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
+      struct alignas(16) Eight { T v[8]; } e = *reinterpret_cast<const Eight *>(src + (d0 < a.D ? d0 : 0));
+      if (d0 >= a.D) memset(&e, 0, sizeof(e));
+      if constexpr (TERMS == 1) {
+        kv_u32x4 x = __builtin_bit_cast(kv_u32x4, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] ^= a.turn;
+        qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, x);
+      } else {
+        const float sign = a.turn ? -1.f : 1.f;
+        union { kv_bf16x2 p[4]; kv_bf16x8 v; } u[TERMS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          kv_bf16x2 t[TERMS];
+          kv_split2<TERMS>((float)Scalar<T>::load(&e.v[2 * j]) * sign, (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign, t);
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) qf[c][s][i] = u[i].v;
+      }
+    }
+  }
+}
+
+// Of sixteen keys: their page, and whether it is there.  Behind the context page 0 stands in.
+struct KvPage { uint32_t id; bool there; };
+struct KvScales { float k, v; bool there; };
+__device__ __forceinline__ KvPage kv_page(const KvAttnArgs &a, uint32_t entry, int key, int len) {
+  const bool there = key < len && entry < a.pages;
+  return KvPage{there ? entry : 0u, there};
+}
+__device__ __forceinline__ KvScales kv_scales(const KvAttnArgs &a, KvPage p, int kvh) {
+  const int64_t ph = (int64_t)p.id * a.Hkv + kvh;
+  return KvScales{a.k_scale[ph], a.v_scale[ph], p.there};
+}
+
+// A running softmax over steps: per column its maximum and this lane's share of the sum, and the 16 features x 16 columns tiles of values.
+template <int VT, int NC> struct KvState {
+  kv_f32x4 o[NC][VT];
+  float m[NC], l[NC];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      m[c] = kNoScore;
+      l[c] = 0.f;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) o[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+};
+// A step's scores s to weights pf, the state to their maximum.  Both scales go into the exponent: with x = s ks and y = x + log2(vs), exp2(y - m) is the
+// weight times vs, and the sum of a lane's sixteen over vs is their share of the softmax's.  edge: some column does not see all of the step.
+template <int VT, int NC, int TERMS>
+__device__ __forceinline__ void kv_weights(kv_f32x4 (&s)[NC][4], KvState<VT, NC> &z, const KvColumns<NC> &k, const KvScales &sc, float scale_log2, int key0, bool edge,
+                                           kv_bf16x8 (&pf)[NC][2][TERMS]) {
+  const float ks = sc.k * scale_log2, vs = sc.there && sc.v > 0.f ? sc.v : 1.f;
+  // log2(vs): its exponent, to which the logarithm of a power of two adds nothing
+  const uint32_t bits = __float_as_uint(vs);
+  const float up_v = (float)((int)(bits >> 23) - 127) + __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)), over_v = __builtin_amdgcn_rcpf(vs);
+  const float times = edge ? 1.f : ks;
+  float top[NC];
+  bool grows = false;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (edge)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = key0 + 4 * t + j;
+          s[c][t][j] = key <= k.hi[c] && key >= k.lo[c] && sc.there ? s[c][t][j] * ks : -INFINITY;
+        }
+    float most = s[c][0][0];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = fmaxf(most, s[c][t][j]);
+    top[c] = column_max(fmaxf(most * times, kNoScore));   // (times is not negative: a negative scale's sign is the queries')
+    grows |= top[c] > z.m[c] + 8.f;
+  }
+  // a maximum that grew by less than 2^8 waits: weights stay below 2^8, and sums in f32 lose nothing by it
+  if (__any(grows)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float up = fmaxf(z.m[c], top[c]), f = __builtin_amdgcn_exp2f(z.m[c] - up);
+      z.m[c] = up;
+      z.l[c] *= f;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) z.o[c][t] *= f;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float down = up_v - z.m[c];
+    float p[16], sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(s[c][t][j], times, down));
+        sum += p[4 * t + j];
+      }
+    z.l[c] = fmaf(sum, over_v, z.l[c]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      union { kv_bf16x2 p[4]; kv_bf16x8 v; } f[TERMS];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        kv_bf16x2 t[TERMS];
+        kv_split2<TERMS>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], t);
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) f[i].p[j] = t[i];
+      }
+#pragma unroll
+      for (int i = 0; i < TERMS; ++i) pf[c][u][i] = f[i].v;
+    }
+  }
+}
+// A tile's columns to the output, or (part >= 0) to the parts, from row `part` on.  l: the whole sums.
+template <typename T, int VT, int NC> __device__ __forceinline__ void kv_store(const KvAttnArgs &a, const KvColumns<NC> &k, const KvState<VT, NC> &z, int64_t part) {
+  const int col = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (!k.live[c]) continue;
+    if (part >= 0) {
+      const int64_t e = part + c * 16 + col;
+      if (g == 0) {
+        a.part_m[e] = z.m[c];
+        a.part_l[e] = z.l[c];
+      }
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+        if (16 * t < a.features) *reinterpret_cast<kv_f32x4 *>(a.part + e * a.features + 16 * t + 4 * g) = z.o[c][t];
+      continue;
+    }
+    const float f = z.l[c] == 0.f ? 0.f : 1.f / z.l[c];
+    T *dst = (T *)a.out + ((int64_t)k.rows[c] * a.Hq + k.heads[c]) * a.D + 4 * g;
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+      struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], z.l[c] == 0.f ? 0.f : z.o[c][t][j] * f);
+      if (16 * t + 4 * g < a.D) *reinterpret_cast<Four *>(dst + 16 * t) = y;
+    }
+  }
+}
+
+// Blocks go to the XCDs in turn: each XCD gets neighbouring workers, whose keys are often the same.
+__device__ __forceinline__ int kv_block() {
+  const int blocks = gridDim.x * gridDim.y, linear = blockIdx.y * gridDim.x + blockIdx.x;
+  return blocks % 8 == 0 ? linear % 8 * (blocks / 8) + linear / 8 : linear;
+}
+
+// What every wave has asked for or written is there, for all of them.
+__device__ __forceinline__ void kv_meet() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Few columns: 16 to a tile, KW waves that share its steps in turn and merge through LDS.
+// The columns of a request and key head are its new tokens times the query heads of the group, G to a token.  A step is 64 keys:
 //     S^T = K . Q^T   (four tiles of 16 keys x 16 columns),      O^T = V^T . P^T   (VT tiles of 16 features x 16 columns)
 // on v_mfma_f32_16x16x32_bf16.  Row 4 g + r of score tile t is key 16 g + 4 t + r of the step, so that the lane group g (lanes 16 g ..) holds
 // the scores of sixteen neighbouring keys, which are the 16 bytes that it loads of a feature of V: the weights are the second product's
 // fragments as they lie in registers, and every load of the cache is 16 bytes a lane, straight to registers.  Sixteen keys lie in one
-// page, so a lane group has one page and one scale of keys and of values; both go into the exponent: with x = s ks and y = x + log2(vs),
-// exp2(y - m) is the weight times vs, and the sum of sixteen of them over vs is their share of the softmax's.
-// KW waves share a tile's steps in turn and merge through LDS; with KW = 1 a wave is a worker by itself and blocks are four of them.
-template <typename T, int FMT, int VT, int NC, int KW>
-__global__ void __launch_bounds__(256, NC * VT <= 8 ? 2 : 1) k_kv_attention(KvAttnArgs a) {
-  constexpr int TERMS = KvTerms<T>::n, QT = 16 * NC, KL = VT / 4, KR = VT % 4;   // 16-byte loads of a key's features; features left
-  constexpr int KS = 2 * KL + (KR == 0 ? 0 : KR == 3 ? 2 : 1);                     // products along the features
-  constexpr int KN = KL + (KR == 3);                                               // whole 16-byte loads
-  constexpr bool TAIL = KR == 1 || KR == 2;                                        // and one of 8 bytes
-  constexpr int WPB = 4 / KW;                                                      // workers of a block
-  constexpr bool HOIST = NC > 1 && VT <= 8 && TERMS == 1;
+// page, so a lane group has one page and one scale of keys and of values.
+template <typename T, int FMT, int VT, int KW>
+__global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 / KW) k_kv_attention(KvAttnArgs a) {
+  typedef KvFeatures<VT> Fe;
+  constexpr int TERMS = KvTerms<T>::n, QT = 16, KS = Fe::KS, KN = Fe::KN;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Blocks go to the XCDs in turn: each gets neighbouring workers, whose keys are often the same.
-  const int blocks = gridDim.x * gridDim.y, linear = blockIdx.y * gridDim.x + blockIdx.x;
-  const int place = blocks % 8 == 0 ? linear % 8 * (blocks / 8) + linear / 8 : linear;
-  const int kvh = place / gridDim.x, worker = place % gridDim.x * WPB + (KW == 1 ? w : 0);
-
-  // ------------------------------------------------ this worker's first request and tile, and how far its share goes
-  // Every wave sums over the requests by itself, 64 at a time, without LDS or barriers: tiles, if each is a worker's, or their units.  (The code
-  // is kept short all through: a wave runs most of it once, at the rate at which instructions arrive.)
-  KvRequest req;
-  int r = -1, tile = 0;
-  int64_t from = 0, left = 1, share = 1, tile_at = 0;   // `from` units of the tile are others'; tile_at: units before the tile
-  {
-    KvRequest x;
-    int64_t own = 0, upto = 0, total = 0, u = worker;
-    for (int pass = 0; pass < 2 && r < 0; ++pass) {
-      int64_t at = 0;
-#pragma unroll 1
-      for (int i = 0; i < a.R; i += 64) {
-        if (pass == 0 || a.R > 64) {
-          x.tiles = 0;
-          if (i + lane < a.R) x = kv_request<QT>(a, i + lane);
-          own = a.workers == 0 ? x.tiles : x.tiles ? kv_units_before(a, x, x.tiles) : 0;
-          upto = at + wave_scan(own, lane);
-        }
-        const uint64_t here = __ballot(pass == 1 && u < upto);
-        if (here) {
-          const int f = __builtin_ctzll(here);
-          r = i + f;
-          tile_at = lane_of(upto - own, f);
-          req.start = __builtin_amdgcn_readlane(x.start, f);
-          req.n = __builtin_amdgcn_readlane(x.n, f);
-          req.len = __builtin_amdgcn_readlane(x.len, f);
-          req.first = __builtin_amdgcn_readlane(x.first, f);
-          req.tiles = __builtin_amdgcn_readlane(x.tiles, f);
-          break;
-        }
-        at = lane_of(upto, 63);
-      }
-      if (pass == 0) {
-        total = at;
-        if (a.workers) {
-          share = max((int64_t)((double)total * a.per_worker) + 1, (int64_t)a.least * kUnits);   // times the workers: no less than the total
-          u = worker * share;
-          if ((KW == 1 ? lane : threadIdx.x) == 0) a.join[(int64_t)kvh * a.workers + worker].first = -1;
-        }
-        if (u >= total) return;
-      }
-    }
-    if (r < 0) return;
-    if (a.workers) {
-      int lo = 0, hi = req.tiles - 1;   // the tile that unit u lies in
-#pragma unroll 1
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (kv_units_before(a, req, mid) <= u - tile_at) lo = mid;
-        else hi = mid - 1;
-      }
-      tile = lo;
-      tile_at += kv_units_before(a, req, tile);
-      from = u - tile_at;
-      left = min(share, total - u);
-    } else {
-      tile = (int)(u - tile_at);
-      left = kv_units(a, req, tile);
-    }
-  }
+  const int place = kv_block(), kvh = place / gridDim.x, worker = place % gridDim.x;
+  KvWork k;
+  if (!kv_deal<QT>(a, kvh, worker, &k)) return;
 
   const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
   const int slot_mask = (1 << a.page_shift) - 1, k_group = col >> 2;
@@ -242,129 +470,69 @@ __global__ void __launch_bounds__(256, NC * VT <= 8 ? 2 : 1) k_kv_attention(KvAt
 #pragma unroll
   for (int t = 0; t < VT; ++t) v_at[t] = (16 * t + col < a.features ? 16 * t + col : 0) << a.page_shift;
 
-  bool first = true;   // of the worker's tiles
-  for (;; first = false) {
-    // ---------------------------------------------- the tile: its columns, the steps of it that are this worker's
-    const int64_t size = kv_units(a, req, tile), to = min(size, from + left);
-    const int len = req.len, columns = req.n * a.G;
-    int rows[NC], heads[NC], hi[NC], lo[NC];
-    bool live[NC];
-    // how far token i sees: keys lo .. hi
-    auto token = [&](int x) { return (int)(((double)x + 0.5) * a.per_group); };
-    auto newest = [&](int i) { return min(max(req.first + i, -1), len - 1); };
-    auto oldest = [&](int i) { return max(max(req.first + i, -1) - a.window + 1, 0); };
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int x = tile * QT + c * 16 + col;
-      live[c] = x < columns;
-      const int i = live[c] ? token(x) : 0;   // (a column behind the last repeats the first, and goes nowhere)
-      rows[c] = req.start + i;
-      heads[c] = kvh * a.G + (live[c] ? x - i * a.G : 0);
-      hi[c] = live[c] ? newest(i) : -1;
-      lo[c] = oldest(i);
-    }
+  for (bool first = true;; first = false) {
+    const int64_t size = kv_units(a, k.req, k.tile), to = min(size, k.from + k.left);
+    const int len = k.req.len, columns = k.req.n * a.G;
+    const KvSeen see = {k.req.first, len, a.window, a.per_group};
+    const KvColumns<1> cols = kv_columns<1>(a, k.req, see, kvh, k.tile * QT, columns);
     // of the tile's first and last token: every live column sees lo_last .. hi_first, none sees outside lo_first .. hi_last
-    const int i_first = token(tile * QT), i_last = token(min((tile + 1) * QT, columns) - 1);
-    const int hi_first = newest(i_first), hi_last = newest(i_last), lo_first = oldest(i_first), lo_last = oldest(i_last);
+    const int i_first = see.token(k.tile * QT), i_last = see.token(min((k.tile + 1) * QT, columns) - 1);
+    const int hi_first = see.newest(i_first), hi_last = see.newest(i_last), lo_first = see.oldest(i_first), lo_last = see.oldest(i_last);
     const int step0 = lo_first / kStep, steps = hi_last >= lo_first ? hi_last / kStep + 1 - step0 : 0;
-    const int s_begin = step0 + (int)min((int64_t)steps, from / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, to / kUnits));
+    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - a.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - a.extra, (int64_t)0) / kUnits));
 
-    kv_bf16x8 qf[NC][KS][TERMS];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const T *src = (const T *)a.q + (int64_t)rows[c] * a.q_row + (int64_t)heads[c] * a.q_head;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d0 = TAIL && s == KS - 1 ? KN * 64 + 8 * g : (s / 2) * 64 + 16 * g + 8 * (s & 1);
-        struct alignas(16) Eight { T v[8]; } e = *reinterpret_cast<const Eight *>(src + (d0 < a.D ? d0 : 0));
-        if (d0 >= a.D) memset(&e, 0, sizeof(e));
-        if constexpr (TERMS == 1) {
-          qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, e);
-        } else {
-          union { kv_bf16x2 p[4]; kv_bf16x8 v; } u[TERMS];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            kv_bf16x2 t[TERMS];
-            kv_split2<TERMS>((float)Scalar<T>::load(&e.v[2 * j]), (float)Scalar<T>::load(&e.v[2 * j + 1]), t);
-#pragma unroll
-            for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
-          }
-#pragma unroll
-          for (int i = 0; i < TERMS; ++i) qf[c][s][i] = u[i].v;
-        }
-      }
-    }
+    kv_bf16x8 qf[1][KS][TERMS];
+    kv_queries<T, VT, 1>(a, cols, qf);
 
-    // ---------------------------------------------- the cache
-    const uint32_t *const table = a.tables + (int64_t)r * a.table_ld;
-    // Of sixteen keys from `key` on: their page, and whether it is there.  Behind the context page 0 stands in.  An entry is asked for two
-    // steps ahead and looked at one step ahead: looked at sooner, it would wait for the loads that went out with it.
-    struct Page { uint32_t id; bool there; };
+    // An entry of the table is asked for two steps ahead and looked at one step ahead: looked at sooner, it would wait for the loads that went
+    // out with it.  So are scales: what a step hands to the next must not wait for keys.
+    const uint32_t *const table = a.tables + (int64_t)k.r * a.table_ld;
     auto entry_of = [&](int key) __attribute__((always_inline)) { return table[key < len ? key >> a.page_shift : 0]; };
-    auto page_of = [&](uint32_t id, int key) __attribute__((always_inline)) {
-      const bool there = key < len && id < a.pages;
-      return Page{there ? id : 0u, there};
-    };
-    struct Step { kv_u32x4 k[KN ? KN : 1][4]; kv_u32x2 tail[4]; kv_u32x4 v[VT]; };
-    struct Scales { float k, v; bool there; };
-    Step now;
-    auto scales_of = [&](Page pv) __attribute__((always_inline)) {
-      const int64_t ph = (int64_t)pv.id * a.Hkv + kvh;
-      return Scales{a.k_scale[ph], a.v_scale[ph], pv.there};
-    };
-    auto load_keys = [&](int st, Page pk) __attribute__((always_inline)) {
-      Step &s = now;
+    struct { kv_u32x4 k[KN ? KN : 1][4]; kv_u32x2 tail[4]; kv_u32x4 v[VT]; } now;
+    auto load_keys = [&](int st, KvPage p) __attribute__((always_inline)) {
       const int key = st * kStep + 16 * k_group + (col & 3);
-      const uint8_t *base = a.k + ((int64_t)pk.id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * a.features;
+      const uint8_t *base = a.k + ((int64_t)p.id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * a.features;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int i = 0; i < KN; ++i) s.k[i][t] = fetch<KW != 1>(base + 4 * t * a.features + k_at[i]);
-        if (TAIL) s.tail[t] = *reinterpret_cast<const kv_u32x2 *>(base + 4 * t * a.features + tail_at);
+        for (int i = 0; i < KN; ++i) now.k[i][t] = fetch_once(base + 4 * t * a.features + k_at[i]);
+        if (Fe::TAIL) now.tail[t] = *reinterpret_cast<const kv_u32x2 *>(base + 4 * t * a.features + tail_at);
       }
     };
-    auto load_values = [&](int st, Page pv) __attribute__((always_inline)) {
-      const uint8_t *values = a.v + ((int64_t)pv.id * a.Hkv + kvh) * head_bytes + ((st * kStep + 16 * g) & slot_mask);
+    auto load_values = [&](int st, KvPage p) __attribute__((always_inline)) {
+      const uint8_t *values = a.v + ((int64_t)p.id * a.Hkv + kvh) * head_bytes + ((st * kStep + 16 * g) & slot_mask);
 #pragma unroll
-      for (int t = 0; t < VT; ++t) now.v[t] = fetch<KW != 1>(values + v_at[t]);
+      for (int t = 0; t < VT; ++t) now.v[t] = fetch_once(values + v_at[t]);
     };
 
-    kv_f32x4 o[NC][VT];
-    float m[NC], l[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      m[c] = kNoScore;
-      l[c] = 0.f;
-#pragma unroll
-      for (int t = 0; t < VT; ++t) o[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    int st = s_begin + (KW == 1 ? 0 : w);
+    KvState<VT, 1> z;
+    z.clear();
+    int st = s_begin + w;
     bool missing = false;
     if (st < s_end) {
       const int last = s_end - 1;
       int next = min(st + KW, last);
       uint32_t nk = entry_of(st * kStep + 16 * k_group), nv = entry_of(st * kStep + 16 * g);
-      Scales scales;
+      KvScales scales;
       {
-        const Page pk = page_of(nk, st * kStep + 16 * k_group), pv = page_of(nv, st * kStep + 16 * g);
+        const KvPage pk = kv_page(a, nk, st * kStep + 16 * k_group, len), pv = kv_page(a, nv, st * kStep + 16 * g, len);
         nk = entry_of(next * kStep + 16 * k_group);
         nv = entry_of(next * kStep + 16 * g);
-        scales = scales_of(pv);
+        scales = kv_scales(a, pv, kvh);
         load_keys(st, pk);
         load_values(st, pv);
       }
       for (; st < s_end; st += KW) {
         const int ahead = min(next + KW, last);
         const uint32_t ak = entry_of(ahead * kStep + 16 * k_group), av = entry_of(ahead * kStep + 16 * g);
-        const Page of_k = page_of(nk, next * kStep + 16 * k_group), of_v = page_of(nv, next * kStep + 16 * g);
-        const Scales coming = scales_of(of_v);   // (ahead of the keys: what a step hands to the next must not wait for those)
+        const KvPage of_k = kv_page(a, nk, next * kStep + 16 * k_group, len), of_v = kv_page(a, nv, next * kStep + 16 * g, len);
+        const KvScales coming = kv_scales(a, of_v, kvh);
         const int key0 = st * kStep + 16 * g;   // this lane group's first
-        const bool there = scales.there, gone = key0 < len && !there;
+        const bool gone = key0 < len && !scales.there;
         missing |= gone;
         if ((st + 1) * kStep > len || __any(gone)) {
           // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
-          const int valid = there ? (int)min(len - key0, (int64_t)16) : 0;
+          const int valid = scales.there ? min(len - key0, 16) : 0;
           uint32_t keep[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -376,117 +544,31 @@ __global__ void __launch_bounds__(256, NC * VT <= 8 ? 2 : 1) k_kv_attention(KvAt
 #pragma unroll
             for (int j = 0; j < 4; ++j) now.v[t][j] &= keep[j];
         }
-        kv_f32x4 s[NC][4];
+        kv_f32x4 s[1][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) s[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+          s[0][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int e = 0; e < KS; ++e) {
             kv_bf16x8 f;
-            if (TAIL && e == KS - 1) f = kv_unpack<FMT>(now.tail[t].x, now.tail[t].y);
+            if (Fe::TAIL && e == KS - 1) f = kv_unpack<FMT>(now.tail[t].x, now.tail[t].y);
             else f = kv_unpack<FMT>(now.k[e / 2][t][2 * (e & 1)], now.k[e / 2][t][2 * (e & 1) + 1]);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-              for (int i = 0; i < TERMS; ++i) s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[c][e][i], s[c][t], 0, 0, 0);
+            for (int i = 0; i < TERMS; ++i) s[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[0][e][i], s[0][t], 0, 0, 0);
           }
         }
-        // With several tiles to share them V's fragments are made here, beside the scores' products, and its registers are free for the next step's
-        kv_bf16x8 vf[HOIST ? VT : 1][2];
-        if constexpr (HOIST) {
-#pragma unroll
-          for (int t = 0; t < VT; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) vf[t][u] = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
-        }
-        const float ks = scales.k * a.scale_log2, vs = there && scales.v > 0.f ? scales.v : 1.f;
         load_keys(next, of_k);
-        if constexpr (HOIST) load_values(next, of_v);
-
-        // log2(vs): its exponent, to which the logarithm of a power of two adds nothing
-        const uint32_t bits = __float_as_uint(vs);
-        const float up_v = (float)((int)(bits >> 23) - 127) + __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)), over_v = __builtin_amdgcn_rcpf(vs);
-        const bool edge = (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone);
-        const float times = edge ? 1.f : ks;
-        float top[NC];
-        bool grows = false;
+        kv_bf16x8 pf[1][2][TERMS];
+        kv_weights<VT, 1, TERMS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone), pf);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (edge)
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int key = key0 + 4 * t + j;
-                s[c][t][j] = key <= hi[c] && key >= lo[c] && there ? s[c][t][j] * ks : -INFINITY;
-              }
-          float most = s[c][0][0], least = s[c][0][0];
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) most = fmaxf(most, s[c][t][j]), least = fminf(least, s[c][t][j]);
-          top[c] = column_max(fmaxf(times < 0.f ? least * times : most * times, kNoScore));
-          grows |= top[c] > m[c] + 8.f;
-        }
-        // a maximum that grew by less than 2^8 waits: weights stay below 2^8, and sums in f32 lose nothing by it
-        if (__any(grows)) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const float up = fmaxf(m[c], top[c]), f = __builtin_amdgcn_exp2f(m[c] - up);
-            m[c] = up;
-            l[c] *= f;
-#pragma unroll
-            for (int t = 0; t < VT; ++t) o[c][t] *= f;
-          }
-        }
-        kv_bf16x8 pf[NC][2][TERMS];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float down = up_v - m[c];
-          float p[16], sum = 0.f;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(s[c][t][j], times, down));
-              sum += p[4 * t + j];
-            }
-          l[c] = fmaf(sum, over_v, l[c]);
+        for (int t = 0; t < VT; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            union { kv_bf16x2 p[4]; kv_bf16x8 v; } f[TERMS];
+            const kv_bf16x8 f = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              kv_bf16x2 t[TERMS];
-              kv_split2<TERMS>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], t);
-#pragma unroll
-              for (int i = 0; i < TERMS; ++i) f[i].p[j] = t[i];
-            }
-#pragma unroll
-            for (int i = 0; i < TERMS; ++i) pf[c][u][i] = f[i].v;
+            for (int i = 0; i < TERMS; ++i) z.o[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[0][u][i], z.o[0][t], 0, 0, 0);
           }
-          if constexpr (HOIST)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int i = 0; i < TERMS; ++i) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t][u], pf[c][u][i], o[c][t], 0, 0, 0);
-        }
-        if constexpr (!HOIST) {
-#pragma unroll
-          for (int t = 0; t < VT; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const kv_bf16x8 f = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
-#pragma unroll
-              for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int i = 0; i < TERMS; ++i) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], o[c][t], 0, 0, 0);
-            }
-          load_values(next, of_v);
-        }
+        load_values(next, of_v);
         next = ahead;
         nk = ak;
         nv = av;
@@ -494,94 +576,215 @@ __global__ void __launch_bounds__(256, NC * VT <= 8 ? 2 : 1) k_kv_attention(KvAt
       }
     }
     if (kvh == 0) {
-      const bool past = from == 0 && tile == 0 && (KW == 1 || w == 0) && a.lens[r] > a.M << a.page_shift;
+      const bool past = k.from == 0 && k.tile == 0 && w == 0 && a.lens[k.r] > a.M << a.page_shift;
       if ((__any(missing) || past) && lane == 0) atomicAdd(a.errors, 1ull);
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) l[c] = column_sum(l[c]);
+    z.l[0] = column_sum(z.l[0]);
 
-    if constexpr (KW > 1) {
-      // the upper half of the waves hands its sums to the lower, until one is left; values lie in LDS as in registers
-      static_assert(NC == 1, "waves that share steps have one tile of 16 columns");
-      __shared__ kv_f32x4 sums[KW / 2][VT][64];
-      __shared__ float stats[KW / 2][2][64];
+    // the upper half of the waves hands its sums to the lower, until one is left; values lie in LDS as in registers
+    __shared__ kv_f32x4 sums[KW / 2][VT][64];
+    __shared__ float stats[KW / 2][2][64];
 #pragma unroll
-      for (int half = KW / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (w >= half && w < 2 * half) {
+    for (int half = KW / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (w >= half && w < 2 * half) {
 #pragma unroll
-          for (int t = 0; t < VT; ++t) sums[w - half][t][lane] = o[0][t];
-          stats[w - half][0][lane] = m[0];
-          stats[w - half][1][lane] = l[0];
-        }
-        __syncthreads();
-        if (w < half) {
-          const float m2 = stats[w][0][lane], l2 = stats[w][1][lane], up = fmaxf(m[0], m2);
-          const float f1 = __builtin_amdgcn_exp2f(m[0] - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
-          m[0] = up;
-          l[0] = l[0] * f1 + l2 * f2;
+        for (int t = 0; t < VT; ++t) sums[w - half][t][lane] = z.o[0][t];
+        stats[w - half][0][lane] = z.m[0];
+        stats[w - half][1][lane] = z.l[0];
+      }
+      __syncthreads();
+      if (w < half) {
+        const float m2 = stats[w][0][lane], l2 = stats[w][1][lane], up = fmaxf(z.m[0], m2);
+        const float f1 = __builtin_amdgcn_exp2f(z.m[0] - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
+        z.m[0] = up;
+        z.l[0] = z.l[0] * f1 + l2 * f2;
 #pragma unroll
-          for (int t = 0; t < VT; ++t) o[0][t] = o[0][t] * f1 + sums[w][t][lane] * f2;
-        }
+        for (int t = 0; t < VT; ++t) z.o[0][t] = z.o[0][t] * f1 + sums[w][t][lane] * f2;
       }
     }
-
-    // ---------------------------------------------- out, or to the tile's other parts
-    const bool whole = from == 0 && to == size;
-    if (KW == 1 || w == 0) {
-      const int64_t own = (int64_t)kvh * a.workers + worker, part = (2 * own + !first) * QT;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (!live[c]) continue;
-        if (!whole) {
-          const int64_t e = part + c * 16 + col;
-          if (g == 0) {
-            a.part_m[e] = m[c];
-            a.part_l[e] = l[c];
-          }
-#pragma unroll
-          for (int t = 0; t < VT; ++t)
-            if (16 * t < a.features) *reinterpret_cast<kv_f32x4 *>(a.part + e * a.features + 16 * t + 4 * g) = o[c][t];
-          continue;
-        }
-        const float f = l[c] == 0.f ? 0.f : 1.f / l[c];
-        T *dst = (T *)a.out + ((int64_t)rows[c] * a.Hq + heads[c]) * a.D + 4 * g;
-#pragma unroll
-        for (int t = 0; t < VT; ++t) {
-          struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], l[c] == 0.f ? 0.f : o[c][t][j] * f);
-          if (16 * t + 4 * g < a.D) *reinterpret_cast<Four *>(dst + 16 * t) = y;
-        }
-      }
-      if (!whole && to == size && lane == 0) {
-        int64_t begin = (int64_t)((double)tile_at / (double)share);
-        begin += begin * share > tile_at ? -1 : (begin + 1) * share <= tile_at ? 1 : 0;
-        a.join[own] = KvJoin{(int)begin, tile_at != begin * share, req.start, tile * QT, min(QT, columns - tile * QT)};
-      }
+    if (w == 0) {
+      const bool whole = k.from == 0 && to == size;
+      const int64_t own = (int64_t)kvh * a.workers + worker;
+      kv_store<T, VT, 1>(a, cols, z, whole ? -1 : (2 * own + !first) * QT);
+      if (!whole && to == size && lane == 0) kv_say_join<QT>(a, k, own, columns);
     }
-    left -= to - from;
-    if (a.workers == 0 || left <= 0) return;
-    from = 0;
-    tile_at += size;
-    if (++tile >= req.tiles) {
-      tile = 0;
-      do {
-        if (++r >= a.R) return;
-        req = kv_request<QT>(a, r);
-      } while (req.tiles == 0);
-    }
+    if (!kv_next<QT>(a, size, to, &k)) return;
   }
 }
 
-// The parts of tiles that workers share, to the output: a block for each worker that had a tile's last part.
+// Many columns: a block of four waves with 16 NC columns each, whose keys and values come through LDS as codes, two buffers, one barrier a step: each
+// byte of the cache reaches a CU once for 64 NC columns, and no register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
+// rows, their 16-byte pieces exchanged so that sixteen rows' reads spread over the banks; values as sixteen keys of a feature.
+template <typename T, int FMT, int VT, int NC>
+__global__ void __launch_bounds__(256, kv_blocks(VT, NC, KvTerms<T>::n)) k_kv_attention_wide(KvAttnArgs a) {
+  typedef KvFeatures<VT> Fe;
+  typedef __attribute__((address_space(3))) void *lds_ptr;
+  constexpr int TERMS = KvTerms<T>::n, QT = 64 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2 * BYTES];   // keys, then values
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int place = kv_block(), kvh = place / gridDim.x, worker = place % gridDim.x;
+  KvWork k;
+  if (!kv_deal<QT>(a, kvh, worker, &k)) return;
+
+  const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
+  const int slot_mask = (1 << a.page_shift) - 1;
+  auto exchange = [](int row) { return VT == 4 ? (row >> 2) & 3 : VT == 8 ? (row >> 1) & 7 : VT == 16 ? row & 15 : 0; };
+  // This lane's pieces of a step, LOADS at most: pieces 64 j .. of wave-sized runs j = w, w + 4, ..: VT runs of keys, VT of values.  `key`: the first
+  // key of the piece within the step, `at`: its bytes from there on.
+  int key_of[LOADS], at_of[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int run = i * 4 + w, piece = (run < VT ? run : run - VT) * 64 + lane;
+    if (run < VT) {
+      const int row = piece / VT, part = (piece % VT) ^ exchange(row), j = row & 15;
+      key_of[i] = 16 * (j >> 2) + 4 * (row >> 4) + (j & 3);
+      at_of[i] = 16 * part < a.features ? 16 * part : 0;
+    } else {
+      const int d = piece % (16 * VT);
+      key_of[i] = 16 * (piece / (16 * VT));
+      at_of[i] = (d < a.features ? d : 0) << a.page_shift;
+    }
+  }
+  int k_at[4];   // this lane's row of score tile t in LDS
+#pragma unroll
+  for (int t = 0; t < 4; ++t) k_at[t] = (16 * t + col) * 16 * VT;
+
+  for (bool first = true;; first = false) {
+    const int64_t size = kv_units(a, k.req, k.tile), to = min(size, k.from + k.left);
+    const int len = k.req.len, columns = k.req.n * a.G;
+    const KvSeen see = {k.req.first, len, a.window, a.per_group};
+    const int x0 = k.tile * QT, xw = x0 + w * 16 * NC;
+    const KvColumns<NC> cols = kv_columns<NC>(a, k.req, see, kvh, xw, columns);
+    // what the tile's first and last token see, for the steps; and this wave's, for what it may skip or need not mask
+    const int i_first = see.token(x0), i_last = see.token(min(x0 + QT, columns) - 1);
+    const int lo_first = see.oldest(i_first), hi_last = see.newest(i_last);
+    const int step0 = lo_first / kStep, steps = hi_last >= lo_first ? hi_last / kStep + 1 - step0 : 0;
+    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - a.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - a.extra, (int64_t)0) / kUnits));
+    const int iw_first = see.token(min(xw, columns - 1)), iw_last = see.token(min(xw + 16 * NC, columns) - 1);
+    const int hi_near = see.newest(iw_first), hi_far = xw < columns ? see.newest(iw_last) : -1, lo_near = see.oldest(iw_last), lo_far = see.oldest(iw_first);
+
+    kv_bf16x8 qf[NC][KS][TERMS];
+    kv_queries<T, VT, NC>(a, cols, qf);
+    const uint32_t *const table = a.tables + (int64_t)k.r * a.table_ld;
+    auto entry_of = [&](int key) __attribute__((always_inline)) { return table[key < len ? key >> a.page_shift : 0]; };
+    auto ask = [&](int st, uint32_t (&e)[LOADS], uint32_t &of_scales) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) e[i] = entry_of(st * kStep + key_of[i]);
+      of_scales = entry_of(st * kStep + 16 * g);
+    };
+    auto load = [&](int st, const uint32_t (&e)[LOADS], uint8_t *to_lds) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int run = i * 4 + w, key = st * kStep + key_of[i];
+        if (LOADS * 4 != 2 * VT && run >= 2 * VT) break;
+        const uint8_t *base = run < VT ? a.k : a.v;
+        base += ((int64_t)kv_page(a, e[i], key, len).id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * (run < VT ? a.features : 1) + at_of[i];
+        __builtin_amdgcn_global_load_lds((const void *)base, (lds_ptr)(to_lds + run * 1024), 16, 0, 0);
+      }
+    };
+
+    KvState<VT, NC> z;
+    z.clear();
+    bool missing = false;
+    if (s_begin < s_end) {
+      const int last = s_end - 1;
+      uint32_t entries[LOADS], e_scales;
+      ask(s_begin, entries, e_scales);
+      KvScales scales = kv_scales(a, kv_page(a, e_scales, s_begin * kStep + 16 * g, len), kvh);
+      kv_meet();   // (nobody reads the tile before any more)
+      load(s_begin, entries, tiles[0]);
+      ask(min(s_begin + 1, last), entries, e_scales);
+      for (int st = s_begin, b = 0; st < s_end; ++st, b ^= 1) {
+        kv_meet();   // this step's pieces, of every wave
+        const int next = min(st + 1, last), key0 = st * kStep + 16 * g;
+        const KvScales coming = kv_scales(a, kv_page(a, e_scales, next * kStep + 16 * g, len), kvh);
+        load(next, entries, tiles[b ^ 1]);
+        ask(min(st + 2, last), entries, e_scales);
+        const bool gone = key0 < len && !scales.there;
+        missing |= gone;
+        uint8_t *const kt = tiles[b], *const vt = tiles[b] + BYTES;
+        if ((st + 1) * kStep > len || __any(gone)) {
+          // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
+          const int valid = scales.there ? min(len - key0, 16) : 0;
+          for (int t = w; t < VT; t += 4) {
+            kv_u32x4 *const p = reinterpret_cast<kv_u32x4 *>(vt + (g * 16 * VT + 16 * t + col) * 16);
+            kv_u32x4 x = *p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int n = min(max(valid - 4 * j, 0), 4);
+              x[j] &= n == 4 ? 0xffffffffu : (1u << 8 * n) - 1;
+            }
+            *p = x;
+          }
+          kv_meet();
+        }
+        if (st * kStep <= hi_far && (st + 1) * kStep > lo_far) {
+          kv_f32x4 s[NC][4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < KS; ++e) {
+              kv_bf16x8 f;
+              if (Fe::TAIL && e == KS - 1) {
+                const int part = min(4 * Fe::KN + (g >> 1), VT - 1) ^ exchange(16 * t + col);
+                const kv_u32x2 x = *reinterpret_cast<const kv_u32x2 *>(kt + k_at[t] + 16 * part + 8 * (g & 1));
+                f = kv_unpack<FMT>(x.x, x.y);
+              } else {
+                const int part = (4 * (e / 2) + g) ^ exchange(16 * t + col);
+                const kv_u32x2 x = *reinterpret_cast<const kv_u32x2 *>(kt + k_at[t] + 16 * part + 8 * (e & 1));
+                f = kv_unpack<FMT>(x.x, x.y);
+              }
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[c][e][i], s[c][t], 0, 0, 0);
+            }
+          }
+          kv_bf16x8 pf[NC][2][TERMS];
+          kv_weights<VT, NC, TERMS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_near || st * kStep < lo_near || __any(gone), pf);
+#pragma unroll
+          for (int t = 0; t < VT; ++t) {
+            const kv_u32x4 v = *reinterpret_cast<const kv_u32x4 *>(vt + (g * 16 * VT + 16 * t + col) * 16);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const kv_bf16x8 f = kv_unpack<FMT>(v[2 * u], v[2 * u + 1]);
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) z.o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], z.o[c][t], 0, 0, 0);
+            }
+          }
+        }
+        scales = coming;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last step asked once more: nothing may land in LDS behind the block's end
+    }
+    if (kvh == 0 && w == 0) {
+      const bool past = k.from == 0 && k.tile == 0 && a.lens[k.r] > a.M << a.page_shift;
+      if ((__any(missing) || past) && lane == 0) atomicAdd(a.errors, 1ull);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) z.l[c] = column_sum(z.l[c]);
+    const bool whole = k.from == 0 && to == size;
+    const int64_t own = (int64_t)kvh * a.workers + worker;
+    kv_store<T, VT, NC>(a, cols, z, whole ? -1 : (2 * own + !first) * QT + w * 16 * NC);
+    if (!whole && to == size && threadIdx.x == 0) kv_say_join<QT>(a, k, own, columns);
+    if (!kv_next<QT>(a, size, to, &k)) return;
+  }
+}
+
+// The parts of tiles that workers share, to the output: a block for each 16 columns of a tile whose last part was a worker's.
 template <typename T> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, int QT) {
   const int64_t worker = blockIdx.x, own = (int64_t)blockIdx.y * a.workers + worker;
   const KvJoin j = a.join[own];
   if (j.first < 0) return;
   const int F4 = a.features / 4;
-  for (int e = threadIdx.x; e < j.columns * F4; e += 256) {
-    const int c = e / F4, d = (e - c * F4) * 4, x = j.column + c, i = x / a.G;
+  const int c0 = blockIdx.z * 16;
+  for (int e = threadIdx.x; e < min(j.columns - c0, 16) * F4; e += 256) {
+    const int c = c0 + e / F4, d = e % F4 * 4, x = j.column + c, i = x / a.G;
     auto part_of = [&](int64_t k) { return (2 * ((int64_t)blockIdx.y * a.workers + k) + (k == j.first ? j.place : 0)) * QT + c; };
     float m = kNoScore, l = 0.f;
     kv_f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -621,8 +824,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv_attention_join
   }
 }
 
-// Tiles of 16 columns to a wave that is a worker by itself: as many as registers hold.
-template <typename T> constexpr int wide_tiles(int features) { return (features <= 128 ? 2 : 1) * (KvTerms<T>::n == 1 ? 2 : 1); }
+// Tiles of 16 columns to a wave of a wide block: as many as registers hold.
+template <typename T> constexpr int wide_tiles(int features) { return KvTerms<T>::n == 1 || (KvTerms<T>::n == 2 && features <= 128) ? 2 : 1; }
 
 // Rows of D features off 16-byte boundaries to ones of F, zeros behind the D; and the other way, of the rows that are a request's.
 struct KvRowsArgs {
@@ -651,37 +854,43 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv_rows_narrow(Kv
   }
 }
 
-// What a launch takes of the scratch: parts of tiles, and the words about them.
-struct KvPlanOfWork {
-  int workers, columns;          // of a key head; of a tile
-  size_t bytes(const KvAttnArgs &a) const { return workers ? (size_t)a.Hkv * workers * (2ll * columns * (a.features + 2) * 4 + sizeof(KvJoin)) : 0; }
+// What a launch takes of the scratch: parts of tiles, and the words about them.  NC = 0: the kernel of few columns.
+template <typename T, int VT, int NC> struct KvShares {
+  static constexpr int QT = NC ? 64 * NC : 16;
+  int workers;                   // of a key head
+  KvShares(const KvAttnArgs &a, int64_t steps) {
+    const int64_t n = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n) / a.Hkv;
+    workers = steps <= kv_alone(NC) ? 0 : n < 1 ? 1 : (int)n;
+  }
+  int64_t parts(const KvAttnArgs &a) const { return 2ll * QT * a.Hkv * workers; }
+  size_t bytes(const KvAttnArgs &a) const { return (size_t)(parts(a) * (a.features + 2) * 4) + (size_t)a.Hkv * workers * sizeof(KvJoin); }
 };
-template <typename T, int VT, int NC, int KW> static KvPlanOfWork plan_of_work(const KvAttnArgs &a, int64_t steps) {
-  constexpr int WPB = 4 / KW;
-  if (steps <= kv_alone(KW)) return {0, 16 * NC};
-  const int64_t workers = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC) * WPB / a.Hkv;
-  return {(int)(workers < WPB ? WPB : workers / WPB * WPB), 16 * NC};
-}
 
-template <typename T, int FMT, int VT, int NC, int KW> static int launch_tiles(hipStream_t st, KvAttnArgs a, int64_t steps, void *ws) {
-  constexpr int QT = 16 * NC, WPB = 4 / KW;
-  const KvPlanOfWork p = plan_of_work<T, VT, NC, KW>(a, steps);
+template <typename T, int FMT, int VT, int NC> static int launch_tiles(hipStream_t st, KvAttnArgs a, int64_t steps, void *ws) {
+  typedef KvShares<T, VT, NC> Shares;
+  constexpr int QT = Shares::QT;
+  const Shares s(a, steps);
   a.each = (16 * QT + a.G - 1) / a.G;
-  a.workers = p.workers;
+  a.extra = kv_extra(NC) * kUnits;
+  a.workers = s.workers;
   if (a.workers) {
-    const int64_t parts = 2 * QT * (int64_t)a.Hkv * a.workers;
-    a.least = kv_least(KW);
+    a.least = kv_least(NC);
     a.per_worker = 1.0 / a.workers;
     a.part = (float *)ws;
-    a.part_m = a.part + parts * a.features;
-    a.part_l = a.part_m + parts;
-    a.join = (KvJoin *)(a.part_l + parts);
+    a.part_m = a.part + s.parts(a) * a.features;
+    a.part_l = a.part_m + s.parts(a);
+    a.join = (KvJoin *)(a.part_l + s.parts(a));
   }
-  const int64_t slots = a.which == 1 ? a.R : a.N * a.G / QT + a.R, x = a.workers ? a.workers / WPB : (slots + WPB - 1) / WPB;
-  hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, NC, KW>), dim3((unsigned)x, (unsigned)a.Hkv), dim3(256), 0, st, a);
+  const int64_t slots = a.which == 1 ? a.R : a.N * a.G / QT + a.R, x = a.workers ? a.workers : slots;
+  const dim3 grid((unsigned)x, (unsigned)a.Hkv);
+  if constexpr (NC > 0) {
+    hipLaunchKernelGGL((k_kv_attention_wide<T, FMT, VT, NC>), grid, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, 4>), grid, dim3(256), 0, st, a);
+  }
   RAI_TRY(launch_check("kv_attention"));
   if (a.workers) {
-    hipLaunchKernelGGL((k_kv_attention_join<T>), dim3((unsigned)a.workers, (unsigned)a.Hkv), dim3(256), 0, st, a, QT);
+    hipLaunchKernelGGL((k_kv_attention_join<T>), dim3(grid.x, grid.y, QT / 16), dim3(256), 0, st, a, QT);
     RAI_TRY(launch_check("kv_attention_join"));
   }
   return RAI_OK;
@@ -690,9 +899,9 @@ template <typename T, int FMT, int VT, int NC, int KW> static int launch_tiles(h
 template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, const KvRowsArgs &odd, bool wide, int64_t steps) {
   constexpr int NC = wide_tiles<T>(16 * VT);
   // the two launches run one after the other and may use the same scratch
-  size_t parts = plan_of_work<T, VT, 1, 4>(a, steps).bytes(a);
+  size_t parts = KvShares<T, VT, 0>(a, steps).bytes(a);
   if (wide) {
-    const size_t others = plan_of_work<T, VT, NC, 1>(a, steps).bytes(a);
+    const size_t others = KvShares<T, VT, NC>(a, steps).bytes(a);
     if (others > parts) parts = others;
   }
   const size_t rows = odd.src ? ((size_t)a.N * a.Hq * a.features * sizeof(T) + 15) / 16 * 16 : 0;
@@ -713,10 +922,10 @@ template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_
   }
   if (wide) {
     a.which = 2;
-    RAI_TRY((launch_tiles<T, FMT, VT, NC, 1>(st, a, steps, ws)));
+    RAI_TRY((launch_tiles<T, FMT, VT, NC>(st, a, steps, ws)));
     a.which = 1;
   }
-  RAI_TRY((launch_tiles<T, FMT, VT, 1, 4>(st, a, steps, ws)));
+  RAI_TRY((launch_tiles<T, FMT, VT, 0>(st, a, steps, ws)));
   if (odd.src) {
     const int64_t blocks = (a.N * a.Hq * odd.D + 255) / 256;
     hipLaunchKernelGGL((k_kv_rows_narrow<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, back);
@@ -797,7 +1006,8 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
     odd.N = N; odd.H = a.Hq; odd.D = a.D; odd.F = a.features; odd.R = a.R;
     odd.starts = a.starts;
   }
-  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.scale_log2 = (float)(fabs(scale) * 1.4426950408889634);
+  a.turn = scale < 0 ? 0x80008000u : 0;
   a.errors = index_error_counter(dev);
 
   a.dev = dev;
