@@ -11,6 +11,25 @@ typedef __attribute__((ext_vector_type(4))) uint32_t kv_u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t kv_u32x2;
 typedef __attribute__((ext_vector_type(2))) float kv_f32x2;
 
+// One of the two kinds of work of a launch: tiles of few columns (16) or of many.
+struct KvKind {
+  int which;                     // requests served: 0 all, 1 those of up to 16 columns, 2 the others
+  int blocks;                    // of the launch
+  int workers;                   // of a key head, each with an even share of the steps; 0: a worker to a tile
+  int each, extra;               // sixteenths of a key that a tile sees more than the one before it, and that its beginning and end are worth
+  int least;                     // steps of a share at least
+  int count;                     // whether the block that leaves a tile's last part joins the parts, or another launch
+  double per_worker;             // 1 / workers
+  float *part;                   // [Hkv * workers][2][columns of a tile][features] sums of a share's first and last tile
+  float *part_m, *part_l;        // their maxima and sums of weights
+  struct KvJoin *join;           // [Hkv * workers]
+};
+// The tile whose last part is a worker's first: workers first .. the worker itself have its parts.
+struct KvJoin {
+  int first;                     // -1: none
+  int place;                     // which of the first worker's two parts
+  int start, column, columns;    // the tile's request's first row, its first column and how many it has
+};
 struct KvAttnArgs {
   const void *q;
   void *out;
@@ -26,23 +45,14 @@ struct KvAttnArgs {
   uint32_t turn;                 // the signs of two bf16 where the scale is negative
   double per_group;              // 1 / G
   int reach;                     // keys that the oldest token of a tile sees, at most
-  int which;                     // requests served: 0 all, 1 those of up to 16 columns, 2 the others
-  int each, extra;               // sixteenths of a key that a tile sees more than the one before it, and that its beginning and end are worth
-  double per_worker;             // 1 / workers
-  int workers;                   // of a key head, each with an even share of the steps; 0: a worker to a tile
-  int least;                     // steps of a share at least
-  float *part;                   // [Hkv * workers][2][columns of a tile][features] sums of a share's first and last tile
-  float *part_m, *part_l;        // their maxima and sums of weights
-  struct KvJoin *join;           // [Hkv * workers]
   unsigned long long *errors;
+  KvKind few, many;
 };
 
-// The tile whose last part is a worker's first: workers first .. the worker itself have its parts.
-struct KvJoin {
-  int first;                     // -1: none
-  int place;                     // which of the first worker's two parts
-  int start, column, columns;    // the tile's request's first row, its first column and how many it has
-};
+// Counts of the workers that have left their part of a tile; the one that counts itself in last joins the parts and sets the count back to
+// zero.  By the first part's place: two to a worker.  Shared by all launches on a device, which run one after the other.
+constexpr int kKvTickets = 1 << 17;
+__device__ int kv_tickets[kKvTickets];
 
 // Eight codes as the eight bf16 of a fragment: every e4m3 value and every whole number up to 127 is a bf16.
 template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, uint32_t hi) {
@@ -108,8 +118,10 @@ constexpr int kv_blocks(int vt, int nc, int terms) { return vt > 8 || (nc > 1 &&
 // Contexts of up to so many steps are not shared between workers; of longer ones a worker has so many at least.
 constexpr int kv_alone(int nc) { return nc ? 8 : 16; }
 constexpr int kv_least(int nc) { return nc ? 2 : 8; }
+// Workers of a key head up to which the last one to leave a tile joins its parts.
+constexpr int kv_counted = 32;
 // Steps that a tile's beginning and end take as long as.
-constexpr int kv_extra(int nc) { return nc ? 2 : 8; }
+constexpr int kv_extra(int nc) { return nc ? 6 : 12; }
 
 // How the work of a key head is dealt out.  A tile of a request is as long as the keys that its last row sees, which grows evenly from tile to
 // tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1), and `extra` for its beginning and end
@@ -120,11 +132,11 @@ struct KvRequest {
   int len, first;                // length, cut to its table's; position of the first new token
 };
 __device__ __forceinline__ int64_t kv_base(const KvAttnArgs &a, const KvRequest &q) { return 16ll * min(max(q.len - q.n, 0), a.reach); }
-__device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return kv_base(a, q) + a.extra + (int64_t)a.each * (tile + 1); }
+__device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvKind &d, const KvRequest &q, int64_t tile) { return kv_base(a, q) + d.extra + (int64_t)d.each * (tile + 1); }
 // of the tiles before `tile`
-__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvRequest &q, int64_t tile) { return tile * (kv_base(a, q) + a.extra) + a.each * (tile * (tile + 1) / 2); }
+__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvKind &d, const KvRequest &q, int64_t tile) { return tile * (kv_base(a, q) + d.extra) + d.each * (tile * (tile + 1) / 2); }
 
-template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, int r) {
+template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, const KvKind &d, int r) {
   KvRequest q;
   const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), said = a.lens[r], most = a.M << a.page_shift;
   q.start = (int)start;
@@ -132,7 +144,7 @@ template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnAr
   q.len = (int)min(max(said, (int64_t)0), most);
   q.first = (int)min(max(said, -(1ll << 30)), most) - q.n;
   const int columns = q.n * a.G;
-  q.tiles = a.which == 1 ? columns > 0 && columns <= 16 : a.which == 2 && columns <= 16 ? 0 : (columns + QT - 1) / QT;
+  q.tiles = d.which == 1 ? columns > 0 && columns <= 16 : d.which == 2 && columns <= 16 ? 0 : (columns + QT - 1) / QT;
   return q;
 }
 __device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
@@ -156,7 +168,7 @@ struct KvWork {
 };
 // Every wave sums over the requests by itself, 64 at a time, without LDS or barriers: tiles, if each is a worker's, or their units.  (The code
 // around the steps is kept short all through: a wave runs it once, at the rate at which instructions arrive.)
-template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, int kvh, int worker, KvWork *out) {
+template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, const KvKind &d, int kvh, int worker, KvWork *out) {
   const int lane = threadIdx.x & 63;
   KvRequest x;
   out->r = -1;
@@ -170,8 +182,8 @@ template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, i
     for (int i = 0; i < a.R; i += 64) {
       if (pass == 0 || a.R > 64) {
         x.tiles = 0;
-        if (i + lane < a.R) x = kv_request<QT>(a, i + lane);
-        own = a.workers == 0 ? x.tiles : x.tiles ? kv_units_before(a, x, x.tiles) : 0;
+        if (i + lane < a.R) x = kv_request<QT>(a, d, i + lane);
+        own = d.workers == 0 ? x.tiles : x.tiles ? kv_units_before(a, d, x, x.tiles) : 0;
         upto = at + wave_scan(own, lane);
       }
       const uint64_t here = __ballot(pass == 1 && u < upto);
@@ -190,55 +202,48 @@ template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, i
     }
     if (pass == 0) {
       total = at;
-      if (a.workers) {
-        out->share = max((int64_t)((double)total * a.per_worker) + 1, (int64_t)a.least * kUnits);   // times the workers: no less than the total
+      if (d.workers) {
+        out->share = max((int64_t)((double)total * d.per_worker) + 1, (int64_t)d.least * kUnits);   // times the workers: no less than the total
         u = worker * out->share;
-        if (threadIdx.x == 0) a.join[(int64_t)kvh * a.workers + worker].first = -1;
+        if (!d.count && threadIdx.x == 0) d.join[(int64_t)kvh * d.workers + worker].first = -1;
       }
       if (u >= total) return false;
     }
   }
   if (out->r < 0) return false;
-  if (a.workers) {
+  if (d.workers) {
     int lo = 0, hi = out->req.tiles - 1;   // the tile that unit u lies in
 #pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (kv_units_before(a, out->req, mid) <= u - out->tile_at) lo = mid;
+      if (kv_units_before(a, d, out->req, mid) <= u - out->tile_at) lo = mid;
       else hi = mid - 1;
     }
     out->tile = lo;
-    out->tile_at += kv_units_before(a, out->req, lo);
+    out->tile_at += kv_units_before(a, d, out->req, lo);
     out->from = u - out->tile_at;
     out->left = min(out->share, total - u);
   } else {
     out->tile = (int)(u - out->tile_at);
-    out->left = kv_units(a, out->req, out->tile);
+    out->left = kv_units(a, d, out->req, out->tile);
   }
   return true;
 }
 // On to the next tile; false behind the worker's last.
-template <int QT> __device__ __forceinline__ bool kv_next(const KvAttnArgs &a, int64_t size, int64_t to, KvWork *k) {
+template <int QT> __device__ __forceinline__ bool kv_next(const KvAttnArgs &a, const KvKind &d, int64_t size, int64_t to, KvWork *k) {
   k->left -= to - k->from;
-  if (a.workers == 0 || k->left <= 0) return false;
+  if (d.workers == 0 || k->left <= 0) return false;
   k->from = 0;
   k->tile_at += size;
   if (++k->tile >= k->req.tiles) {
     k->tile = 0;
     do {
       if (++k->r >= a.R) return false;
-      k->req = kv_request<QT>(a, k->r);
+      k->req = kv_request<QT>(a, d, k->r);
     } while (k->req.tiles == 0);
   }
   return true;
 }
-// The first part of a tile that others finish, or end, is said to the launch that joins them.
-template <int QT> __device__ __forceinline__ void kv_say_join(const KvAttnArgs &a, const KvWork &k, int64_t own, int columns) {
-  int64_t begin = (int64_t)((double)k.tile_at / (double)k.share);
-  begin += begin * k.share > k.tile_at ? -1 : (begin + 1) * k.share <= k.tile_at ? 1 : 0;
-  a.join[own] = KvJoin{(int)begin, k.tile_at != begin * k.share, k.req.start, k.tile * QT, min(QT, columns - k.tile * QT)};
-}
-
 // Which keys the tokens of a request see: of token i, oldest(i) .. newest(i).
 struct KvSeen {
   int first, len, window;
@@ -283,12 +288,14 @@ __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<
 #pragma unroll
     for (int s = 0; s < KvFeatures<VT>::KS; ++s) {
       const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
-      struct alignas(16) Eight { T v[8]; } e = *reinterpret_cast<const Eight *>(src + (d0 < a.D ? d0 : 0));
-      if (d0 >= a.D) memset(&e, 0, sizeof(e));
+      // (no branch: lanes without these features take others and put zeros in their place)
+      struct alignas(16) Eight { T v[8]; };
+      const bool there = d0 < a.D;
+      const Eight e = *reinterpret_cast<const Eight *>(src + (there ? d0 : 0));
       if constexpr (TERMS == 1) {
         kv_u32x4 x = __builtin_bit_cast(kv_u32x4, e);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] ^= a.turn;
+        for (int j = 0; j < 4; ++j) x[j] = there ? x[j] ^ a.turn : 0u;
         qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, x);
       } else {
         const float sign = a.turn ? -1.f : 1.f;
@@ -296,7 +303,7 @@ __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           kv_bf16x2 t[TERMS];
-          kv_split2<TERMS>((float)Scalar<T>::load(&e.v[2 * j]) * sign, (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign, t);
+          kv_split2<TERMS>(there ? (float)Scalar<T>::load(&e.v[2 * j]) * sign : 0.f, there ? (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign : 0.f, t);
 #pragma unroll
           for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
         }
@@ -330,6 +337,17 @@ template <int VT, int NC> struct KvState {
       l[c] = 0.f;
 #pragma unroll
       for (int t = 0; t < VT; ++t) o[c][t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // another's, over other keys of the same columns
+  __device__ __forceinline__ void add(const KvState &y) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float up = fmaxf(m[c], y.m[c]), f1 = __builtin_amdgcn_exp2f(m[c] - up), f2 = __builtin_amdgcn_exp2f(y.m[c] - up);
+      m[c] = up;
+      l[c] = l[c] * f1 + y.l[c] * f2;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) o[c][t] = o[c][t] * f1 + y.o[c][t] * f2;
     }
   }
 };
@@ -401,40 +419,102 @@ __device__ __forceinline__ void kv_weights(kv_f32x4 (&s)[NC][4], KvState<VT, NC>
     }
   }
 }
-// A tile's columns to the output, or (part >= 0) to the parts, from row `part` on.  l: the whole sums.
-template <typename T, int VT, int NC> __device__ __forceinline__ void kv_store(const KvAttnArgs &a, const KvColumns<NC> &k, const KvState<VT, NC> &z, int64_t part) {
+// The L2s of the XCDs are not coherent for ordinary accesses: what blocks hand to one another is written through and read around them.
+__device__ __forceinline__ void kv_put(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float kv_get(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void kv_put4(float *p, kv_f32x4 v) {
+  struct Pair { uint64_t a, b; } x = __builtin_bit_cast(Pair, v);
+  __hip_atomic_store((uint64_t *)p, x.a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((uint64_t *)p + 1, x.b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ kv_f32x4 kv_get4(const float *p) {
+  struct Pair { uint64_t a, b; } x;
+  x.a = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  x.b = __hip_atomic_load((const uint64_t *)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __builtin_bit_cast(kv_f32x4, x);
+}
+
+// The end of a tile, or of a worker's part of one.  The wave holds columns c0 .. of the tile and of their features the tiles t0, t0 + step, ..; held:
+// whether it holds any.  A whole tile goes to the output, a part to the scratch, from where another launch joins them; or (COUNT, d.count)
+// each part is counted in, and the block that counts itself in last, which waits for nobody, joins them and writes the output.  That saves the
+// launch, but reads one part after the other: it serves where a tile has few workers.
+template <typename T, bool COUNT, int OT, int NC>
+__device__ __forceinline__ void kv_finish(const KvAttnArgs &a, const KvKind &d, const KvWork &k, int kvh, int worker, bool first, int64_t size, int64_t to, int QT, int c0, int t0, int step,
+                                          bool held, const KvColumns<NC> &cols, KvState<OT, NC> &z, int *sh_last) {
   const int col = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  auto feature = [&](int i) { return 16 * (t0 + step * i) + 4 * g; };
+  if (k.from != 0 || to != size) {
+    const int64_t own = (int64_t)kvh * d.workers + worker;
+    auto row_of = [&](int64_t place, int c) { return place * QT + c0 + c * 16 + col; };
+    // the workers that have a part: from the one that the tile's first unit is in to the one that its last is in
+    auto worker_of = [&](int64_t u) {
+      int64_t w = (int64_t)((double)u / (double)k.share);
+      return w + (w * k.share > u ? -1 : (w + 1) * k.share <= u ? 1 : 0);
+    };
+    const int64_t begin = worker_of(k.tile_at), place = k.tile_at != begin * k.share;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (!k.live[c]) continue;
-    if (part >= 0) {
-      const int64_t e = part + c * 16 + col;
-      if (g == 0) {
-        a.part_m[e] = z.m[c];
-        a.part_l[e] = z.l[c];
+    for (int c = 0; c < NC; ++c) {
+      if (!cols.live[c] || !held) continue;
+      const int64_t e = row_of(2 * own + !first, c);
+      if (g == 0 && t0 == 0) {
+        kv_put(d.part_m + e, z.m[c]);
+        kv_put(d.part_l + e, z.l[c]);
       }
 #pragma unroll
-      for (int t = 0; t < VT; ++t)
-        if (16 * t < a.features) *reinterpret_cast<kv_f32x4 *>(a.part + e * a.features + 16 * t + 4 * g) = z.o[c][t];
-      continue;
+      for (int i = 0; i < OT; ++i)
+        if (feature(i) < a.features) {
+          float *const p = d.part + e * a.features + feature(i);
+          if (COUNT && d.count) kv_put4(p, z.o[c][i]);
+          else *reinterpret_cast<kv_f32x4 *>(p) = z.o[c][i];
+        }
     }
-    const float f = z.l[c] == 0.f ? 0.f : 1.f / z.l[c];
-    T *dst = (T *)a.out + ((int64_t)k.rows[c] * a.Hq + k.heads[c]) * a.D + 4 * g;
+    if (!COUNT || !d.count) {
+      if (to == size && threadIdx.x == 0) d.join[own] = KvJoin{(int)begin, (int)place, k.req.start, k.tile * QT, min(QT, k.req.n * a.G - k.tile * QT)};
+      return;
+    }
+    const int64_t end = worker_of(k.tile_at + size - 1);
+    int *const ticket = kv_tickets + 2 * ((int64_t)kvh * d.workers + begin) + place;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this thread has written through is there
+    __syncthreads();
+    if (threadIdx.x == 0) *sh_last = atomicAdd(ticket, 1) == end - begin;
+    __syncthreads();
+    const bool last = *sh_last;
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    z.clear();
+    for (int64_t w = begin; w <= end; ++w) {
+      const int64_t at = 2 * ((int64_t)kvh * d.workers + w) + (w == begin ? place : 0);
+      KvState<OT, NC> y;
 #pragma unroll
-    for (int t = 0; t < VT; ++t) {
+      for (int c = 0; c < NC; ++c) {
+        const int64_t e = cols.live[c] ? row_of(at, c) : at * QT;   // (a column that is not there reads the tile's first)
+        y.m[c] = kv_get(d.part_m + e);
+        y.l[c] = kv_get(d.part_l + e);
+#pragma unroll
+        for (int i = 0; i < OT; ++i) y.o[c][i] = kv_get4(d.part + e * a.features + (feature(i) < a.features ? feature(i) : 0));
+      }
+      z.add(y);
+    }
+  }
+  if (!held) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (!cols.live[c]) continue;
+    const float f = z.l[c] == 0.f ? 0.f : 1.f / z.l[c];
+    T *dst = (T *)a.out + ((int64_t)cols.rows[c] * a.Hq + cols.heads[c]) * a.D;
+#pragma unroll
+    for (int i = 0; i < OT; ++i) {
       struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], z.l[c] == 0.f ? 0.f : z.o[c][t][j] * f);
-      if (16 * t + 4 * g < a.D) *reinterpret_cast<Four *>(dst + 16 * t) = y;
+      for (int j = 0; j < 4; ++j) Scalar<T>::store(&y.v[j], z.l[c] == 0.f ? 0.f : z.o[c][i][j] * f);
+      if (feature(i) < a.D) *reinterpret_cast<Four *>(dst + feature(i)) = y;
     }
   }
 }
 
-// Blocks go to the XCDs in turn: each XCD gets neighbouring workers, whose keys are often the same.
-__device__ __forceinline__ int kv_block() {
-  const int blocks = gridDim.x * gridDim.y, linear = blockIdx.y * gridDim.x + blockIdx.x;
-  return blocks % 8 == 0 ? linear % 8 * (blocks / 8) + linear / 8 : linear;
-}
+// Blocks go to the XCDs in turn: each XCD gets neighbouring workers, whose keys are often the same; but not where workers are whole tiles, which
+// are of different lengths from request to request.
+__device__ __forceinline__ int kv_block(const KvKind &d, int block) { return d.workers && d.blocks % 8 == 0 ? block % 8 * (d.blocks / 8) + block / 8 : block; }
 
 // What every wave has asked for or written is there, for all of them.
 __device__ __forceinline__ void kv_meet() {
@@ -450,14 +530,14 @@ __device__ __forceinline__ void kv_meet() {
 // the scores of sixteen neighbouring keys, which are the 16 bytes that it loads of a feature of V: the weights are the second product's
 // fragments as they lie in registers, and every load of the cache is 16 bytes a lane, straight to registers.  Sixteen keys lie in one
 // page, so a lane group has one page and one scale of keys and of values.
-template <typename T, int FMT, int VT, int KW>
-__global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 / KW) k_kv_attention(KvAttnArgs a) {
+template <typename T, int VT> constexpr int kv_few_lds() { return 4 * VT * 64 * 16 + 4 * 2 * 64 * 4; }
+template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
   typedef KvFeatures<VT> Fe;
-  constexpr int TERMS = KvTerms<T>::n, QT = 16, KS = Fe::KS, KN = Fe::KN;
+  constexpr int TERMS = KvTerms<T>::n, QT = 16, KS = Fe::KS, KN = Fe::KN, KW = 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int place = kv_block(), kvh = place / gridDim.x, worker = place % gridDim.x;
+  const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
-  if (!kv_deal<QT>(a, kvh, worker, &k)) return;
+  if (!kv_deal<QT>(a, d, kvh, worker, &k)) return;
 
   const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
   const int slot_mask = (1 << a.page_shift) - 1, k_group = col >> 2;
@@ -471,7 +551,7 @@ __global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 /
   for (int t = 0; t < VT; ++t) v_at[t] = (16 * t + col < a.features ? 16 * t + col : 0) << a.page_shift;
 
   for (bool first = true;; first = false) {
-    const int64_t size = kv_units(a, k.req, k.tile), to = min(size, k.from + k.left);
+    const int64_t size = kv_units(a, d, k.req, k.tile), to = min(size, k.from + k.left);
     const int len = k.req.len, columns = k.req.n * a.G;
     const KvSeen see = {k.req.first, len, a.window, a.per_group};
     const KvColumns<1> cols = kv_columns<1>(a, k.req, see, kvh, k.tile * QT, columns);
@@ -479,10 +559,7 @@ __global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 /
     const int i_first = see.token(k.tile * QT), i_last = see.token(min((k.tile + 1) * QT, columns) - 1);
     const int hi_first = see.newest(i_first), hi_last = see.newest(i_last), lo_first = see.oldest(i_first), lo_last = see.oldest(i_last);
     const int step0 = lo_first / kStep, steps = hi_last >= lo_first ? hi_last / kStep + 1 - step0 : 0;
-    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - a.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - a.extra, (int64_t)0) / kUnits));
-
-    kv_bf16x8 qf[1][KS][TERMS];
-    kv_queries<T, VT, 1>(a, cols, qf);
+    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - d.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - d.extra, (int64_t)0) / kUnits));
 
     // An entry of the table is asked for two steps ahead and looked at one step ahead: looked at sooner, it would wait for the loads that went
     // out with it.  So are scales: what a step hands to the next must not wait for keys.
@@ -522,6 +599,8 @@ __global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 /
         load_keys(st, pk);
         load_values(st, pv);
       }
+      kv_bf16x8 qf[1][KS][TERMS];   // (behind the keys, which would wait for them)
+      kv_queries<T, VT, 1>(a, cols, qf);
       for (; st < s_end; st += KW) {
         const int ahead = min(next + KW, last);
         const uint32_t ak = entry_of(ahead * kStep + 16 * k_group), av = entry_of(ahead * kStep + 16 * g);
@@ -581,51 +660,47 @@ __global__ void __launch_bounds__(64 * KW, kv_blocks(VT, 1, KvTerms<T>::n) * 4 /
     }
     z.l[0] = column_sum(z.l[0]);
 
-    // the upper half of the waves hands its sums to the lower, until one is left; values lie in LDS as in registers
-    __shared__ kv_f32x4 sums[KW / 2][VT][64];
-    __shared__ float stats[KW / 2][2][64];
+    // every wave's sums to LDS as they lie in registers, and every fourth tile of features to a wave
+    constexpr int OT = (VT + 3) / 4;
+    kv_f32x4 (*const sums)[VT][64] = reinterpret_cast<kv_f32x4 (*)[VT][64]>(lds);
+    float (*const stats)[2][64] = reinterpret_cast<float (*)[2][64]>(lds + 4 * VT * 64 * 16);
+    __syncthreads();   // (nobody reads the tile before any more)
 #pragma unroll
-    for (int half = KW / 2; half > 0; half /= 2) {
-      __syncthreads();
-      if (w >= half && w < 2 * half) {
+    for (int t = 0; t < VT; ++t) sums[w][t][lane] = z.o[0][t];
+    stats[w][0][lane] = z.m[0];
+    stats[w][1][lane] = z.l[0];
+    __syncthreads();
+    KvState<OT, 1> y;
+    y.clear();
+    float f[4];
 #pragma unroll
-        for (int t = 0; t < VT; ++t) sums[w - half][t][lane] = z.o[0][t];
-        stats[w - half][0][lane] = z.m[0];
-        stats[w - half][1][lane] = z.l[0];
-      }
-      __syncthreads();
-      if (w < half) {
-        const float m2 = stats[w][0][lane], l2 = stats[w][1][lane], up = fmaxf(z.m[0], m2);
-        const float f1 = __builtin_amdgcn_exp2f(z.m[0] - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
-        z.m[0] = up;
-        z.l[0] = z.l[0] * f1 + l2 * f2;
+    for (int i = 0; i < 4; ++i) y.m[0] = fmaxf(y.m[0], stats[i][0][lane]);
 #pragma unroll
-        for (int t = 0; t < VT; ++t) z.o[0][t] = z.o[0][t] * f1 + sums[w][t][lane] * f2;
-      }
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __builtin_amdgcn_exp2f(stats[i][0][lane] - y.m[0]);
+      y.l[0] = fmaf(stats[i][1][lane], f[i], y.l[0]);
+#pragma unroll
+      for (int t = 0; t < OT; ++t) y.o[0][t] += sums[i][min(4 * t + w, VT - 1)][lane] * f[i];
     }
-    if (w == 0) {
-      const bool whole = k.from == 0 && to == size;
-      const int64_t own = (int64_t)kvh * a.workers + worker;
-      kv_store<T, VT, 1>(a, cols, z, whole ? -1 : (2 * own + !first) * QT);
-      if (!whole && to == size && lane == 0) kv_say_join<QT>(a, k, own, columns);
-    }
-    if (!kv_next<QT>(a, size, to, &k)) return;
+    kv_finish<T, true, OT, 1>(a, d, k, kvh, worker, first, size, to, QT, 0, w, 4, true, cols, y, sh_last);
+    if (!kv_next<QT>(a, d, size, to, &k)) return;
   }
 }
 
-// Many columns: a block of four waves with 16 NC columns each, whose keys and values come through LDS as codes, two buffers, one barrier a step: each
-// byte of the cache reaches a CU once for 64 NC columns, and no register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
+// Many columns: two waves of 16 NC columns each for the even steps of a tile and two for the odd ones, merged through LDS at its end.  Keys and values come
+// through LDS as codes, two buffers of two steps, one barrier for both: each byte of the cache reaches a CU once for 32 NC columns, and no
+// register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
 // rows, their 16-byte pieces exchanged so that sixteen rows' reads spread over the banks; values as sixteen keys of a feature.
-template <typename T, int FMT, int VT, int NC>
-__global__ void __launch_bounds__(256, kv_blocks(VT, NC, KvTerms<T>::n)) k_kv_attention_wide(KvAttnArgs a) {
+template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
+template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
   typedef KvFeatures<VT> Fe;
   typedef __attribute__((address_space(3))) void *lds_ptr;
-  constexpr int TERMS = KvTerms<T>::n, QT = 64 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2 * BYTES];   // keys, then values
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int place = kv_block(), kvh = place / gridDim.x, worker = place % gridDim.x;
+  constexpr int TERMS = KvTerms<T>::n, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
+  uint8_t *const tiles[2] = {lds, lds + 4 * BYTES};   // of two steps: keys, then values
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w >> 1;
+  const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
-  if (!kv_deal<QT>(a, kvh, worker, &k)) return;
+  if (!kv_deal<QT>(a, d, kvh, worker, &k)) return;
 
   const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
   const int slot_mask = (1 << a.page_shift) - 1;
@@ -651,63 +726,69 @@ __global__ void __launch_bounds__(256, kv_blocks(VT, NC, KvTerms<T>::n)) k_kv_at
   for (int t = 0; t < 4; ++t) k_at[t] = (16 * t + col) * 16 * VT;
 
   for (bool first = true;; first = false) {
-    const int64_t size = kv_units(a, k.req, k.tile), to = min(size, k.from + k.left);
+    const int64_t size = kv_units(a, d, k.req, k.tile), to = min(size, k.from + k.left);
     const int len = k.req.len, columns = k.req.n * a.G;
     const KvSeen see = {k.req.first, len, a.window, a.per_group};
-    const int x0 = k.tile * QT, xw = x0 + w * 16 * NC;
+    const int x0 = k.tile * QT, xw = x0 + (w & 1) * 16 * NC;
     const KvColumns<NC> cols = kv_columns<NC>(a, k.req, see, kvh, xw, columns);
     // what the tile's first and last token see, for the steps; and this wave's, for what it may skip or need not mask
     const int i_first = see.token(x0), i_last = see.token(min(x0 + QT, columns) - 1);
     const int lo_first = see.oldest(i_first), hi_last = see.newest(i_last);
     const int step0 = lo_first / kStep, steps = hi_last >= lo_first ? hi_last / kStep + 1 - step0 : 0;
-    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - a.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - a.extra, (int64_t)0) / kUnits));
+    const int s_begin = step0 + (int)min((int64_t)steps, max(k.from - d.extra, (int64_t)0) / kUnits), s_end = step0 + (to == size ? steps : (int)min((int64_t)steps, max(to - d.extra, (int64_t)0) / kUnits));
     const int iw_first = see.token(min(xw, columns - 1)), iw_last = see.token(min(xw + 16 * NC, columns) - 1);
     const int hi_near = see.newest(iw_first), hi_far = xw < columns ? see.newest(iw_last) : -1, lo_near = see.oldest(iw_last), lo_far = see.oldest(iw_first);
 
-    kv_bf16x8 qf[NC][KS][TERMS];
-    kv_queries<T, VT, NC>(a, cols, qf);
     const uint32_t *const table = a.tables + (int64_t)k.r * a.table_ld;
     auto entry_of = [&](int key) __attribute__((always_inline)) { return table[key < len ? key >> a.page_shift : 0]; };
-    auto ask = [&](int st, uint32_t (&e)[LOADS], uint32_t &of_scales) __attribute__((always_inline)) {
+    // the two steps from `st` on; a step behind the last is asked for as the last
+    const int last = s_end - 1;
+    auto ask = [&](int st, uint32_t (&e)[2][LOADS], uint32_t &of_scales) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) e[i] = entry_of(st * kStep + key_of[i]);
-      of_scales = entry_of(st * kStep + 16 * g);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) e[h][i] = entry_of(min(st + h, last) * kStep + key_of[i]);
+      of_scales = entry_of(min(st + half, last) * kStep + 16 * g);
     };
-    auto load = [&](int st, const uint32_t (&e)[LOADS], uint8_t *to_lds) __attribute__((always_inline)) {
+    auto load = [&](int st, const uint32_t (&e)[2][LOADS], uint8_t *to_lds) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int run = i * 4 + w, key = st * kStep + key_of[i];
-        if (LOADS * 4 != 2 * VT && run >= 2 * VT) break;
-        const uint8_t *base = run < VT ? a.k : a.v;
-        base += ((int64_t)kv_page(a, e[i], key, len).id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * (run < VT ? a.features : 1) + at_of[i];
-        __builtin_amdgcn_global_load_lds((const void *)base, (lds_ptr)(to_lds + run * 1024), 16, 0, 0);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int run = i * 4 + w, key = min(st + h, last) * kStep + key_of[i];
+          if (LOADS * 4 != 2 * VT && run >= 2 * VT) break;
+          const uint8_t *base = run < VT ? a.k : a.v;
+          base += ((int64_t)kv_page(a, e[h][i], key, len).id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * (run < VT ? a.features : 1) + at_of[i];
+          __builtin_amdgcn_global_load_lds((const void *)base, (lds_ptr)(to_lds + h * 2 * BYTES + run * 1024), 16, 0, 0);
+        }
     };
 
     KvState<VT, NC> z;
     z.clear();
     bool missing = false;
     if (s_begin < s_end) {
-      const int last = s_end - 1;
-      uint32_t entries[LOADS], e_scales;
+      uint32_t entries[2][LOADS], e_scales;
       ask(s_begin, entries, e_scales);
-      KvScales scales = kv_scales(a, kv_page(a, e_scales, s_begin * kStep + 16 * g, len), kvh);
+      KvScales scales = kv_scales(a, kv_page(a, e_scales, min(s_begin + half, last) * kStep + 16 * g, len), kvh);
       kv_meet();   // (nobody reads the tile before any more)
       load(s_begin, entries, tiles[0]);
-      ask(min(s_begin + 1, last), entries, e_scales);
-      for (int st = s_begin, b = 0; st < s_end; ++st, b ^= 1) {
-        kv_meet();   // this step's pieces, of every wave
-        const int next = min(st + 1, last), key0 = st * kStep + 16 * g;
-        const KvScales coming = kv_scales(a, kv_page(a, e_scales, next * kStep + 16 * g, len), kvh);
+      ask(min(s_begin + 2, last), entries, e_scales);
+      kv_bf16x8 qf[NC][KS][TERMS];
+      kv_queries<T, VT, NC>(a, cols, qf);
+      for (int st0 = s_begin, b = 0; st0 < s_end; st0 += 2, b ^= 1) {
+        kv_meet();   // these steps' pieces, of every wave
+        const int st = st0 + half, next = min(st0 + 2, last), key0 = st * kStep + 16 * g;
+        const KvScales coming = kv_scales(a, kv_page(a, e_scales, min(next + half, last) * kStep + 16 * g, len), kvh);
         load(next, entries, tiles[b ^ 1]);
-        ask(min(st + 2, last), entries, e_scales);
-        const bool gone = key0 < len && !scales.there;
+        ask(min(st0 + 4, last), entries, e_scales);
+        const bool gone = st < s_end && key0 < len && !scales.there;
         missing |= gone;
-        uint8_t *const kt = tiles[b], *const vt = tiles[b] + BYTES;
-        if ((st + 1) * kStep > len || __any(gone)) {
-          // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
+        uint8_t *const kt = tiles[b] + half * 2 * BYTES, *const vt = kt + BYTES;
+        if (st < s_end && ((st + 1) * kStep > len || __any(gone))) {
+          // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be.  (Each wave does it for itself: the
+          // step's other one writes the same.)
           const int valid = scales.there ? min(len - key0, 16) : 0;
-          for (int t = w; t < VT; t += 4) {
+          for (int t = 0; t < VT; ++t) {
             kv_u32x4 *const p = reinterpret_cast<kv_u32x4 *>(vt + (g * 16 * VT + 16 * t + col) * 16);
             kv_u32x4 x = *p;
 #pragma unroll
@@ -717,9 +798,9 @@ __global__ void __launch_bounds__(256, kv_blocks(VT, NC, KvTerms<T>::n)) k_kv_at
             }
             *p = x;
           }
-          kv_meet();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        if (st * kStep <= hi_far && (st + 1) * kStep > lo_far) {
+        if (st < s_end && st * kStep <= hi_far && (st + 1) * kStep > lo_far) {
           kv_f32x4 s[NC][4];
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
@@ -762,66 +843,111 @@ __global__ void __launch_bounds__(256, kv_blocks(VT, NC, KvTerms<T>::n)) k_kv_at
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last step asked once more: nothing may land in LDS behind the block's end
     }
-    if (kvh == 0 && w == 0) {
-      const bool past = k.from == 0 && k.tile == 0 && a.lens[k.r] > a.M << a.page_shift;
+    if (kvh == 0 && (w & 1) == 0) {
+      const bool past = w == 0 && k.from == 0 && k.tile == 0 && a.lens[k.r] > a.M << a.page_shift;
       if ((__any(missing) || past) && lane == 0) atomicAdd(a.errors, 1ull);
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) z.l[c] = column_sum(z.l[c]);
-    const bool whole = k.from == 0 && to == size;
-    const int64_t own = (int64_t)kvh * a.workers + worker;
-    kv_store<T, VT, NC>(a, cols, z, whole ? -1 : (2 * own + !first) * QT + w * 16 * NC);
-    if (!whole && to == size && threadIdx.x == 0) kv_say_join<QT>(a, k, own, columns);
-    if (!kv_next<QT>(a, size, to, &k)) return;
+    // the odd steps' sums to the waves of the even ones, as they lie in registers
+    kv_f32x4 (*const sums)[NC][VT][64] = reinterpret_cast<kv_f32x4 (*)[NC][VT][64]>(lds);
+    float (*const stats)[NC][2][64] = reinterpret_cast<float (*)[NC][2][64]>(lds + 2 * NC * VT * 1024);
+    static_assert(2 * NC * VT * 1024 + 2 * NC * 2 * 256 <= kv_wide_lds<VT>(), "the merge's room");
+    kv_meet();
+    if (half == 1) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+#pragma unroll
+        for (int t = 0; t < VT; ++t) sums[w & 1][c][t][lane] = z.o[c][t];
+        stats[w & 1][c][0][lane] = z.m[c];
+        stats[w & 1][c][1][lane] = z.l[c];
+      }
+    }
+    kv_meet();
+    if (half == 0) {
+      KvState<VT, NC> y;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+#pragma unroll
+        for (int t = 0; t < VT; ++t) y.o[c][t] = sums[w][c][t][lane];
+        y.m[c] = stats[w][c][0][lane];
+        y.l[c] = stats[w][c][1][lane];
+      }
+      z.add(y);
+    }
+    kv_finish<T, false, VT, NC>(a, d, k, kvh, worker, first, size, to, QT, (w & 1) * 16 * NC, 0, 1, half == 0, cols, z, sh_last);
+    if (!kv_next<QT>(a, d, size, to, &k)) return;
   }
 }
 
-// The parts of tiles that workers share, to the output: a block for each 16 columns of a tile whose last part was a worker's.
-template <typename T> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, int QT) {
-  const int64_t worker = blockIdx.x, own = (int64_t)blockIdx.y * a.workers + worker;
-  const KvJoin j = a.join[own];
-  if (j.first < 0) return;
-  const int F4 = a.features / 4;
-  const int c0 = blockIdx.z * 16;
-  for (int e = threadIdx.x; e < min(j.columns - c0, 16) * F4; e += 256) {
-    const int c = c0 + e / F4, d = e % F4 * 4, x = j.column + c, i = x / a.G;
-    auto part_of = [&](int64_t k) { return (2 * ((int64_t)blockIdx.y * a.workers + k) + (k == j.first ? j.place : 0)) * QT + c; };
-    float m = kNoScore, l = 0.f;
-    kv_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t k = j.first; k <= worker; k += 4) {   // four parts asked for at a time
-      float pm[4], pl[4], up = m;
-      kv_f32x4 y[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t p = part_of(min(k + u, worker));
-        pm[u] = a.part_m[p];
-        pl[u] = a.part_l[p];
-        y[u] = *reinterpret_cast<const kv_f32x4 *>(a.part + p * a.features + d);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (k + u > worker) pm[u] = kNoScore, pl[u] = 0.f, y[u] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
-        up = fmaxf(up, pm[u]);
-      }
-      const float f = __builtin_amdgcn_exp2f(m - up);
-      l *= f;
-      o *= f;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float g = __builtin_amdgcn_exp2f(pm[u] - up);
-        l = fmaf(pl[u], g, l);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = fmaf(y[u][v], g, o[v]);
-      }
-      m = up;
+// Requests of few columns and those of many in one launch, the larger work first.  NC = 0: no request has many.
+template <typename T, int FMT, int VT, int NC>
+__global__ void __launch_bounds__(256, kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n)) k_kv_attention(KvAttnArgs a) {
+  constexpr int FEW = kv_few_lds<T, VT>(), WIDE = NC ? kv_wide_lds<VT>() : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[FEW > WIDE ? FEW : WIDE];
+  __shared__ int sh_last;
+  if constexpr (NC > 0) {
+    if ((int)blockIdx.x < a.many.blocks) {
+      kv_wide<T, FMT, VT, NC>(a, a.many, blockIdx.x, lds, &sh_last);
+      return;
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    T *dst = (T *)a.out + (((int64_t)j.start + i) * a.Hq + (int64_t)blockIdx.y * a.G + x - i * a.G) * a.D + d;
-    struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) Scalar<T>::store(&y.v[u], l == 0.f ? 0.f : o[u] * f);
-    if (d < a.D) *reinterpret_cast<Four *>(dst) = y;
   }
+  kv_few<T, FMT, VT>(a, a.few, blockIdx.x - (NC ? a.many.blocks : 0), lds, &sh_last);
+}
+
+// The parts of tiles that workers share, to the output.  Blocks for each worker that had a tile's last part, over the tile's columns: a wave reads whole rows of
+// as many columns as fit it.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
+template <typename T, bool PARTS> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, KvKind d, int QT) {
+  __shared__ kv_f32x4 sums[4][64];
+  __shared__ float stats[4][2][64];
+  const int worker = blockIdx.x, kvh = blockIdx.y;
+  const int64_t base = (int64_t)kvh * d.workers;
+  const KvJoin j = d.join[base + worker];
+  const int F4 = a.features / 4, per_wave = 64 / F4, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = (PARTS ? blockIdx.z : blockIdx.z * 4 + w) * per_wave + lane / F4, f = lane % F4 * 4;
+  const bool live = j.first >= 0 && lane / F4 < per_wave && c < j.columns;
+  if (j.first < 0 || (PARTS && (int)blockIdx.z * per_wave >= j.columns)) return;
+  const int cc = live ? c : 0;
+  float m = kNoScore, l = 0.f;
+  kv_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float pm, float pl, kv_f32x4 y) __attribute__((always_inline)) {
+    const float up = fmaxf(m, pm), f1 = __builtin_amdgcn_exp2f(m - up), f2 = __builtin_amdgcn_exp2f(pm - up);
+    m = up;
+    l = l * f1 + pl * f2;
+    o = o * f1 + y * f2;
+  };
+  constexpr int AT_ONCE = 4, STEP = PARTS ? 4 : 1;
+  for (int k = j.first + (PARTS ? w : 0); k <= worker; k += AT_ONCE * STEP) {
+    float pm[AT_ONCE], pl[AT_ONCE];
+    kv_f32x4 y[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int p = min(k + u * STEP, worker);
+      const int64_t row = (2 * (base + p) + (p == j.first ? j.place : 0)) * QT + cc;
+      pm[u] = k + u * STEP <= worker ? d.part_m[row] : kNoScore;
+      pl[u] = k + u * STEP <= worker ? d.part_l[row] : 0.f;
+      y[u] = *reinterpret_cast<const kv_f32x4 *>(d.part + row * a.features + f);
+      if (k + u * STEP > worker) y[u] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) add(pm[u], pl[u], y[u]);
+  }
+  if constexpr (PARTS) {
+    sums[w][lane] = o;
+    stats[w][0][lane] = m;
+    stats[w][1][lane] = l;
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int u = 1; u < 4; ++u) add(stats[u][0][lane], stats[u][1][lane], sums[u][lane]);
+  }
+  if (!live || f >= a.D) return;
+  const int x = j.column + c, i = x / a.G;
+  const float over = l == 0.f ? 0.f : 1.f / l;
+  struct alignas(sizeof(T) * 4) Four { T v[4]; } y;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) Scalar<T>::store(&y.v[u], l == 0.f ? 0.f : o[u] * over);
+  *reinterpret_cast<Four *>((T *)a.out + (((int64_t)j.start + i) * a.Hq + (int64_t)kvh * a.G + x - i * a.G) * a.D + f) = y;
 }
 
 // Tiles of 16 columns to a wave of a wide block: as many as registers hold.
@@ -854,65 +980,51 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv_rows_narrow(Kv
   }
 }
 
-// What a launch takes of the scratch: parts of tiles, and the words about them.  NC = 0: the kernel of few columns.
+// A kind's workers and what it takes of the scratch.
 template <typename T, int VT, int NC> struct KvShares {
-  static constexpr int QT = NC ? 64 * NC : 16;
-  int workers;                   // of a key head
+  static constexpr int QT = NC ? 32 * NC : 16;
+  int workers;
+  int64_t parts;
   KvShares(const KvAttnArgs &a, int64_t steps) {
-    const int64_t n = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n) / a.Hkv;
+    const int64_t slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n), n = slots / a.Hkv;
     workers = steps <= kv_alone(NC) ? 0 : n < 1 ? 1 : (int)n;
+    parts = 2ll * QT * a.Hkv * workers;
   }
-  int64_t parts(const KvAttnArgs &a) const { return 2ll * QT * a.Hkv * workers; }
-  size_t bytes(const KvAttnArgs &a) const { return (size_t)(parts(a) * (a.features + 2) * 4) + (size_t)a.Hkv * workers * sizeof(KvJoin); }
+  size_t bytes(const KvAttnArgs &a) const { return (size_t)(parts * (a.features + 2) * 4) + (size_t)a.Hkv * workers * sizeof(KvJoin); }
+  KvKind kind(const KvAttnArgs &a, int which, void *ws) const {
+    KvKind d;
+    memset(&d, 0, sizeof(d));
+    d.which = which;
+    d.workers = workers;
+    d.blocks = (workers ? workers : (int)(which == 1 ? a.R : a.N * a.G / QT + a.R)) * a.Hkv;
+    d.each = (16 * QT + a.G - 1) / a.G;
+    d.extra = kv_extra(NC) * kUnits;
+    d.least = kv_least(NC);
+    d.count = NC == 0 && workers <= kv_counted && 2 * a.Hkv * workers <= kKvTickets;
+    d.per_worker = workers ? 1.0 / workers : 0;
+    d.part = (float *)ws;
+    d.part_m = d.part + parts * a.features;
+    d.part_l = d.part_m + parts;
+    d.join = (KvJoin *)(d.part_l + parts);
+    return d;
+  }
 };
-
-template <typename T, int FMT, int VT, int NC> static int launch_tiles(hipStream_t st, KvAttnArgs a, int64_t steps, void *ws) {
-  typedef KvShares<T, VT, NC> Shares;
-  constexpr int QT = Shares::QT;
-  const Shares s(a, steps);
-  a.each = (16 * QT + a.G - 1) / a.G;
-  a.extra = kv_extra(NC) * kUnits;
-  a.workers = s.workers;
-  if (a.workers) {
-    a.least = kv_least(NC);
-    a.per_worker = 1.0 / a.workers;
-    a.part = (float *)ws;
-    a.part_m = a.part + s.parts(a) * a.features;
-    a.part_l = a.part_m + s.parts(a);
-    a.join = (KvJoin *)(a.part_l + s.parts(a));
-  }
-  const int64_t slots = a.which == 1 ? a.R : a.N * a.G / QT + a.R, x = a.workers ? a.workers : slots;
-  const dim3 grid((unsigned)x, (unsigned)a.Hkv);
-  if constexpr (NC > 0) {
-    hipLaunchKernelGGL((k_kv_attention_wide<T, FMT, VT, NC>), grid, dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, 4>), grid, dim3(256), 0, st, a);
-  }
-  RAI_TRY(launch_check("kv_attention"));
-  if (a.workers) {
-    hipLaunchKernelGGL((k_kv_attention_join<T>), dim3(grid.x, grid.y, QT / 16), dim3(256), 0, st, a, QT);
-    RAI_TRY(launch_check("kv_attention_join"));
-  }
-  return RAI_OK;
-}
 
 template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, const KvRowsArgs &odd, bool wide, int64_t steps) {
   constexpr int NC = wide_tiles<T>(16 * VT);
-  // the two launches run one after the other and may use the same scratch
-  size_t parts = KvShares<T, VT, 0>(a, steps).bytes(a);
-  if (wide) {
-    const size_t others = KvShares<T, VT, NC>(a, steps).bytes(a);
-    if (others > parts) parts = others;
-  }
+  const KvShares<T, VT, 0> few(a, steps);
+  const KvShares<T, VT, NC> many(a, steps);
+  const size_t of_few = few.bytes(a), of_many = wide ? many.bytes(a) : 0;
   const size_t rows = odd.src ? ((size_t)a.N * a.Hq * a.features * sizeof(T) + 15) / 16 * 16 : 0;
   WorkspaceHold hold;
   void *ws = nullptr;
-  if (parts + rows) RAI_TRY(workspace(a.dev, parts + 2 * rows, &ws, &hold));
+  if (of_few + of_many + rows) RAI_TRY(workspace(a.dev, of_few + of_many + 2 * rows, &ws, &hold));
+  char *const base = (char *)ws;
   const int64_t most = kNumCU * 32;
   KvRowsArgs in = odd, back = odd;
   if (odd.src) {
-    a.q = in.dst = (char *)ws + parts;
-    a.out = (char *)ws + parts + rows;
+    a.q = in.dst = base;
+    a.out = base + rows;
     back.src = a.out;
     a.q_row = (int64_t)a.Hq * a.features;
     a.q_head = a.D = a.features;
@@ -920,12 +1032,27 @@ template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_
     hipLaunchKernelGGL((k_kv_rows_widen<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, in);
     RAI_TRY(launch_check("kv_rows_widen"));
   }
+  a.few = few.kind(a, wide ? 1 : 0, base + 2 * rows);
+  if (wide) a.many = many.kind(a, 2, base + 2 * rows + of_few);
+  dim3 grid;
+  RAI_TRY(grid_of_blocks((int64_t)a.few.blocks + a.many.blocks, 256, &grid));
+  RAI_REQUIRE(grid.y == 1, RAI_ERR_UNSUPPORTED, "kv_attention: %d blocks", a.few.blocks + a.many.blocks);
   if (wide) {
-    a.which = 2;
-    RAI_TRY((launch_tiles<T, FMT, VT, NC>(st, a, steps, ws)));
-    a.which = 1;
+    hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, NC>), grid, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, 0>), grid, dim3(256), 0, st, a);
   }
-  RAI_TRY((launch_tiles<T, FMT, VT, 0>(st, a, steps, ws)));
+  RAI_TRY(launch_check("kv_attention"));
+  const int per_wave = 256 / a.features;
+  if (a.few.workers && !a.few.count) {
+    hipLaunchKernelGGL((k_kv_attention_join<T, true>), dim3((unsigned)a.few.workers, (unsigned)a.Hkv, (unsigned)((few.QT + per_wave - 1) / per_wave)), dim3(256), 0, st, a, a.few, few.QT);
+    RAI_TRY(launch_check("kv_attention_join"));
+  }
+  if (a.many.workers) {
+    hipLaunchKernelGGL((k_kv_attention_join<T, false>), dim3((unsigned)a.many.workers, (unsigned)a.Hkv, (unsigned)((many.QT + 4 * per_wave - 1) / (4 * per_wave))), dim3(256), 0, st, a,
+                       a.many, many.QT);
+    RAI_TRY(launch_check("kv_attention_join"));
+  }
   if (odd.src) {
     const int64_t blocks = (a.N * a.Hq * odd.D + 255) / 256;
     hipLaunchKernelGGL((k_kv_rows_narrow<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, back);
