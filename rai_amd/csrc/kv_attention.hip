@@ -39,7 +39,7 @@ struct KvAttnArgs {
   const int64_t *starts, *lens;
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
-  int64_t pages;
+  uint32_t pages;
   int dev, R, Hq, Hkv, G, D, features, page_shift, window;
   float scale_log2;              // |scale| * log2(e)
   uint32_t turn;                 // the signs of two bf16 where the scale is negative
@@ -279,23 +279,29 @@ template <int VT> struct KvFeatures {
   static constexpr bool TAIL = KR == 1 || KR == 2;
   static __device__ __forceinline__ int of_product(int s, int g) { return TAIL && s == KS - 1 ? KN * 64 + 8 * g : (s / 2) * 64 + 16 * g + 8 * (s & 1); }
 };
-template <typename T, int VT, int NC>
+template <typename T, int VT, int NC, bool TOGETHER>
 __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<NC> &k, kv_bf16x8 (&qf)[NC][KvFeatures<VT>::KS][KvTerms<T>::n]) {
-  constexpr int TERMS = KvTerms<T>::n;
+  constexpr int TERMS = KvTerms<T>::n, KS = KvFeatures<VT>::KS;
+  struct alignas(16) Eight { T v[8]; } all[NC][KS];
+  // (no branch: lanes without these features take others and put zeros in their place)
+  bool there[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
+    there[s] = d0 < a.D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) all[c][s] = *reinterpret_cast<const Eight *>((const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head + (there[s] ? d0 : 0));
+  }
+  if (TOGETHER) __builtin_amdgcn_sched_barrier(0);   // all on their way before the first is waited for
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const T *src = (const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head;
 #pragma unroll
-    for (int s = 0; s < KvFeatures<VT>::KS; ++s) {
-      const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
-      // (no branch: lanes without these features take others and put zeros in their place)
-      struct alignas(16) Eight { T v[8]; };
-      const bool there = d0 < a.D;
-      const Eight e = *reinterpret_cast<const Eight *>(src + (there ? d0 : 0));
+    for (int s = 0; s < KS; ++s) {
+      const Eight e = all[c][s];
       if constexpr (TERMS == 1) {
         kv_u32x4 x = __builtin_bit_cast(kv_u32x4, e);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = there ? x[j] ^ a.turn : 0u;
+        for (int j = 0; j < 4; ++j) x[j] = there[s] ? x[j] ^ a.turn : 0u;
         qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, x);
       } else {
         const float sign = a.turn ? -1.f : 1.f;
@@ -303,7 +309,7 @@ __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           kv_bf16x2 t[TERMS];
-          kv_split2<TERMS>(there ? (float)Scalar<T>::load(&e.v[2 * j]) * sign : 0.f, there ? (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign : 0.f, t);
+          kv_split2<TERMS>(there[s] ? (float)Scalar<T>::load(&e.v[2 * j]) * sign : 0.f, there[s] ? (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign : 0.f, t);
 #pragma unroll
           for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
         }
@@ -539,7 +545,8 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
   KvWork k;
   if (!kv_deal<QT>(a, d, kvh, worker, &k)) return;
 
-  const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
+  const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features, page_bytes = a.Hkv * head_bytes;
+  const uint8_t *const keys = a.k + kvh * head_bytes, *const values = a.v + kvh * head_bytes;
   const int slot_mask = (1 << a.page_shift) - 1, k_group = col >> 2;
   // Features behind the cache's last are read again from its beginning: q is zero there.
   int k_at[KN ? KN : 1];
@@ -568,7 +575,7 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
     struct { kv_u32x4 k[KN ? KN : 1][4]; kv_u32x2 tail[4]; kv_u32x4 v[VT]; } now;
     auto load_keys = [&](int st, KvPage p) __attribute__((always_inline)) {
       const int key = st * kStep + 16 * k_group + (col & 3);
-      const uint8_t *base = a.k + ((int64_t)p.id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * a.features;
+      const uint8_t *base = keys + (int64_t)p.id * page_bytes + (key & slot_mask) * a.features;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -577,9 +584,9 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
       }
     };
     auto load_values = [&](int st, KvPage p) __attribute__((always_inline)) {
-      const uint8_t *values = a.v + ((int64_t)p.id * a.Hkv + kvh) * head_bytes + ((st * kStep + 16 * g) & slot_mask);
+      const uint8_t *base = values + (int64_t)p.id * page_bytes + ((st * kStep + 16 * g) & slot_mask);
 #pragma unroll
-      for (int t = 0; t < VT; ++t) now.v[t] = fetch_once(values + v_at[t]);
+      for (int t = 0; t < VT; ++t) now.v[t] = fetch_once(base + v_at[t]);
     };
 
     KvState<VT, 1> z;
@@ -600,7 +607,7 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
         load_values(st, pv);
       }
       kv_bf16x8 qf[1][KS][TERMS];   // (behind the keys, which would wait for them)
-      kv_queries<T, VT, 1>(a, cols, qf);
+      kv_queries<T, VT, 1, false>(a, cols, qf);
       for (; st < s_end; st += KW) {
         const int ahead = min(next + KW, last);
         const uint32_t ak = entry_of(ahead * kStep + 16 * k_group), av = entry_of(ahead * kStep + 16 * g);
@@ -687,6 +694,12 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
   }
 }
 
+// 16 bytes a lane straight to LDS, at `to` (the wave's) + 16 * lane.  Not by the builtin, behind which the compiler puts a wait for all that is on its way before the
+// next read of LDS, of the other buffer too: kv_meet waits, before a barrier.  The instruction writes no register.
+__device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(to), "v"(from) : "memory");
+}
+
 // Many columns: two waves of 16 NC columns each for the even steps of a tile and two for the odd ones, merged through LDS at its end.  Keys and values come
 // through LDS as codes, two buffers of two steps, one barrier for both: each byte of the cache reaches a CU once for 32 NC columns, and no
 // register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
@@ -694,36 +707,43 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
 template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
   typedef KvFeatures<VT> Fe;
-  typedef __attribute__((address_space(3))) void *lds_ptr;
   constexpr int TERMS = KvTerms<T>::n, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
-  uint8_t *const tiles[2] = {lds, lds + 4 * BYTES};   // of two steps: keys, then values
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w >> 1;
   const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
   if (!kv_deal<QT>(a, d, kvh, worker, &k)) return;
 
-  const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features;
+  const int64_t head_bytes = ((int64_t)1 << a.page_shift) * a.features, page_bytes = a.Hkv * head_bytes;
+  const uint8_t *const keys = a.k + kvh * head_bytes, *const values = a.v + kvh * head_bytes;
   const int slot_mask = (1 << a.page_shift) - 1;
-  auto exchange = [](int row) { return VT == 4 ? (row >> 2) & 3 : VT == 8 ? (row >> 1) & 7 : VT == 16 ? row & 15 : 0; };
-  // This lane's pieces of a step, LOADS at most: pieces 64 j .. of wave-sized runs j = w, w + 4, ..: VT runs of keys, VT of values.  `key`: the first
-  // key of the piece within the step, `at`: its bytes from there on.
-  int key_of[LOADS], at_of[LOADS];
+  // A step's pieces of 16 bytes are asked for in runs of 64, VT runs of keys and VT of values, every fourth a wave's.  Where VT is a multiple of 4 a run
+  // lies in sixteen keys (KEYED: keys in their order in LDS), a wave's i-th run of values in the same as its i-th of keys, so that their page and first byte are
+  // found by scalar instructions, once for both, and a lane adds an offset that does not change; else each lane finds its own, and keys lie in the order
+  // of the score tiles' rows.  Found by lane all through, addresses took as many instructions as everything between the products.
+  constexpr bool KEYED = VT % 4 == 0;
+  constexpr int ASKS = KEYED ? VT / 4 : LOADS;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+  auto exchange = [](int column) { return VT == 4 ? column >> 2 : VT == 8 ? column >> 1 : VT == 16 ? column : 0; };
+  int key_of[ASKS], at_of[LOADS];   // first key of the piece (KEYED: of its run), bytes from there on
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int run = i * 4 + w, piece = (run < VT ? run : run - VT) * 64 + lane;
     if (run < VT) {
-      const int row = piece / VT, part = (piece % VT) ^ exchange(row), j = row & 15;
-      key_of[i] = 16 * (j >> 2) + 4 * (row >> 4) + (j & 3);
-      at_of[i] = 16 * part < a.features ? 16 * part : 0;
+      const int row = piece / VT, j = KEYED ? (row & 3) | (row >> 4) << 2 : row & 15, part = (piece % VT) ^ exchange(j);
+      if (!KEYED) key_of[i % ASKS] = 16 * (j >> 2) + 4 * (row >> 4) + (j & 3);
+      at_of[i] = (KEYED ? row % 16 * a.features : 0) + (16 * part < a.features ? 16 * part : 0);
     } else {
       const int d = piece % (16 * VT);
-      key_of[i] = 16 * (piece / (16 * VT));
+      if (!KEYED) key_of[i % ASKS] = 16 * (piece / (16 * VT));
       at_of[i] = (d < a.features ? d : 0) << a.page_shift;
     }
   }
+  if (KEYED)
+#pragma unroll
+    for (int i = 0; i < ASKS; ++i) key_of[i] = (i * 4 + w) * 4 / VT * 16;
   int k_at[4];   // this lane's row of score tile t in LDS
 #pragma unroll
-  for (int t = 0; t < 4; ++t) k_at[t] = (16 * t + col) * 16 * VT;
+  for (int t = 0; t < 4; ++t) k_at[t] = (KEYED ? 16 * (col >> 2) + 4 * t + (col & 3) : 16 * t + col) * 16 * VT;
 
   for (bool first = true;; first = false) {
     const int64_t size = kv_units(a, d, k.req, k.tile), to = min(size, k.from + k.left);
@@ -743,47 +763,56 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
     auto entry_of = [&](int key) __attribute__((always_inline)) { return table[key < len ? key >> a.page_shift : 0]; };
     // the two steps from `st` on; a step behind the last is asked for as the last
     const int last = s_end - 1;
-    auto ask = [&](int st, uint32_t (&e)[2][LOADS], uint32_t &of_scales) __attribute__((always_inline)) {
+    auto ask = [&](int st, uint32_t (&e)[2][ASKS], uint32_t &of_scales) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) e[h][i] = entry_of(min(st + h, last) * kStep + key_of[i]);
+        for (int i = 0; i < ASKS; ++i) {
+          const int key = min(st + h, last) * kStep + key_of[i];
+          if constexpr (KEYED) e[h][i] = ((const __attribute__((address_space(4))) uint32_t *)table)[key < len ? key >> a.page_shift : 0];
+          else e[h][i] = entry_of(key);
+        }
       of_scales = entry_of(min(st + half, last) * kStep + 16 * g);
     };
-    auto load = [&](int st, const uint32_t (&e)[2][LOADS], uint8_t *to_lds) __attribute__((always_inline)) {
+    auto load = [&](int st, const uint32_t (&e)[2][ASKS], uint32_t to_lds) __attribute__((always_inline)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int run = i * 4 + w, key = min(st + h, last) * kStep + key_of[i];
-          if (LOADS * 4 != 2 * VT && run >= 2 * VT) break;
-          const uint8_t *base = run < VT ? a.k : a.v;
-          base += ((int64_t)kv_page(a, e[h][i], key, len).id * a.Hkv + kvh) * head_bytes + (key & slot_mask) * (run < VT ? a.features : 1) + at_of[i];
-          __builtin_amdgcn_global_load_lds((const void *)base, (lds_ptr)(to_lds + h * 2 * BYTES + run * 1024), 16, 0, 0);
+        for (int i = 0; i < ASKS; ++i) {
+          const int run = i * 4 + w, key = min(st + h, last) * kStep + key_of[i], slot = key & slot_mask;
+          const int64_t page = (int64_t)kv_page(a, e[h][i], key, len).id * page_bytes;
+          if constexpr (KEYED) {
+            kv_to_lds(keys + (page + slot * a.features) + at_of[i], to_lds + h * 2 * BYTES + run * 1024);
+            kv_to_lds(values + (page + slot) + at_of[i + ASKS], to_lds + h * 2 * BYTES + (VT + run) * 1024);
+          } else {
+            if (run >= 2 * VT) break;
+            kv_to_lds((run < VT ? keys : values) + page + slot * (run < VT ? a.features : 1) + at_of[i], to_lds + h * 2 * BYTES + run * 1024);
+          }
         }
+      }
     };
 
     KvState<VT, NC> z;
     z.clear();
     bool missing = false;
     if (s_begin < s_end) {
-      uint32_t entries[2][LOADS], e_scales;
+      uint32_t entries[2][ASKS], e_scales;
       ask(s_begin, entries, e_scales);
       KvScales scales = kv_scales(a, kv_page(a, e_scales, min(s_begin + half, last) * kStep + 16 * g, len), kvh);
       kv_meet();   // (nobody reads the tile before any more)
-      load(s_begin, entries, tiles[0]);
+      load(s_begin, entries, lds_at);
       ask(min(s_begin + 2, last), entries, e_scales);
       kv_bf16x8 qf[NC][KS][TERMS];
-      kv_queries<T, VT, NC>(a, cols, qf);
+      kv_queries<T, VT, NC, true>(a, cols, qf);
       for (int st0 = s_begin, b = 0; st0 < s_end; st0 += 2, b ^= 1) {
         kv_meet();   // these steps' pieces, of every wave
         const int st = st0 + half, next = min(st0 + 2, last), key0 = st * kStep + 16 * g;
         const KvScales coming = kv_scales(a, kv_page(a, e_scales, min(next + half, last) * kStep + 16 * g, len), kvh);
-        load(next, entries, tiles[b ^ 1]);
+        load(next, entries, lds_at + (b ^ 1) * 4 * BYTES);
         ask(min(st0 + 4, last), entries, e_scales);
         const bool gone = st < s_end && key0 < len && !scales.there;
         missing |= gone;
-        uint8_t *const kt = tiles[b] + half * 2 * BYTES, *const vt = kt + BYTES;
+        uint8_t *const kt = lds + (b * 4 + half * 2) * BYTES, *const vt = kt + BYTES;
         if (st < s_end && ((st + 1) * kStep > len || __any(gone))) {
           // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be.  (Each wave does it for itself: the
           // step's other one writes the same.)
@@ -810,11 +839,11 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
             for (int e = 0; e < KS; ++e) {
               kv_bf16x8 f;
               if (Fe::TAIL && e == KS - 1) {
-                const int part = min(4 * Fe::KN + (g >> 1), VT - 1) ^ exchange(16 * t + col);
+                const int part = min(4 * Fe::KN + (g >> 1), VT - 1) ^ exchange(col);
                 const kv_u32x2 x = *reinterpret_cast<const kv_u32x2 *>(kt + k_at[t] + 16 * part + 8 * (g & 1));
                 f = kv_unpack<FMT>(x.x, x.y);
               } else {
-                const int part = (4 * (e / 2) + g) ^ exchange(16 * t + col);
+                const int part = (4 * (e / 2) + g) ^ exchange(col);
                 const kv_u32x2 x = *reinterpret_cast<const kv_u32x2 *>(kt + k_at[t] + 16 * part + 8 * (e & 1));
                 f = kv_unpack<FMT>(x.x, x.y);
               }
@@ -1115,7 +1144,7 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
   a.starts = (const int64_t *)base_ptr(starts);
   a.lens = (const int64_t *)base_ptr(lens);
   a.k = c.k; a.v = c.v; a.k_scale = c.k_scale; a.v_scale = c.v_scale;
-  a.pages = M == 0 ? 0 : c.pages;
+  a.pages = (uint32_t)(M == 0 ? 0 : c.pages < (int64_t)UINT32_MAX ? c.pages : (int64_t)UINT32_MAX);
   a.R = (int)R; a.Hq = (int)Hq; a.Hkv = c.heads; a.G = (int)(Hq / c.heads); a.D = (int)D;
   a.features = c.features; a.page_shift = c.page_shift;
   a.window = window > 0 ? window : INT32_MAX;
