@@ -115,8 +115,12 @@ constexpr int kStep = 64;                      // keys of a step
 
 // Blocks of a kernel that a CU holds.
 constexpr int kv_blocks(int vt, int nc, int terms) { return vt > 8 || (nc > 1 && terms > 1 && vt > 4) ? 1 : nc > 1 || vt > 5 || terms > 1 ? 2 : 3; }
-// Contexts of up to so many steps are not shared between workers; of longer ones a worker has so many at least.
-constexpr int kv_alone(int nc) { return nc ? 8 : 16; }
+// Tiles of up to so many steps are not shared between workers; `full`: where tiles as they are keep half the card busy.  Measured, whole against shared: of
+// few columns, 16 requests of up to 1200 keys over 8 heads (19 steps) 16 us against 22 and of up to 2048 over 32 heads (32, full) 26 against 33, but one of
+// 2048 over 32 heads (not full) 19 against 14, and 16 of up to 4000 (63, full) 40 against 38; of many, a window of 512 keys (10) 38 against 42, 16 chunks of up
+// to 256 behind up to 700 (11) 28 against 43, 8 of up to 1024 with nothing before (16) 56 against 62, but a window of 1024 (18) 57 against 51.
+constexpr int kv_alone(int nc, bool full) { return nc ? 16 : full ? 40 : 24; }
+// Steps of a share at least.
 constexpr int kv_least(int nc) { return nc ? 2 : 8; }
 // Workers of a key head up to which the last one to leave a tile joins its parts.
 constexpr int kv_counted = 32;
@@ -1014,9 +1018,11 @@ template <typename T, int VT, int NC> struct KvShares {
   static constexpr int QT = NC ? 32 * NC : 16;
   int workers;
   int64_t parts;
-  KvShares(const KvAttnArgs &a, int64_t steps) {
-    const int64_t slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n), n = slots / a.Hkv;
-    workers = steps <= kv_alone(NC) ? 0 : n < 1 ? 1 : (int)n;
+  // tiles: as many as there may be.  No more workers than the least share allows: blocks that find nothing to do take their time too.
+  KvShares(const KvAttnArgs &a, int64_t steps, int64_t tiles) {
+    const int64_t slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n) / a.Hkv, useful = (tiles * (steps + kv_extra(NC)) + kv_least(NC) - 1) / kv_least(NC);
+    const int64_t n = slots < useful ? slots : useful;
+    workers = steps <= kv_alone(NC, 2 * tiles >= slots) ? 0 : n < 1 ? 1 : (int)n;
     parts = 2ll * QT * a.Hkv * workers;
   }
   size_t bytes(const KvAttnArgs &a) const { return (size_t)(parts * (a.features + 2) * 4) + (size_t)a.Hkv * workers * sizeof(KvJoin); }
@@ -1041,8 +1047,8 @@ template <typename T, int VT, int NC> struct KvShares {
 
 template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, const KvRowsArgs &odd, bool wide, int64_t steps) {
   constexpr int NC = wide_tiles<T>(16 * VT);
-  const KvShares<T, VT, 0> few(a, steps);
-  const KvShares<T, VT, NC> many(a, steps);
+  const KvShares<T, VT, 0> few(a, steps, wide ? a.R : a.N * a.G / 16 + a.R);
+  const KvShares<T, VT, NC> many(a, steps, a.N * a.G / (32 * NC) + a.R);
   const size_t of_few = few.bytes(a), of_many = wide ? many.bytes(a) : 0;
   const size_t rows = odd.src ? ((size_t)a.N * a.Hq * a.features * sizeof(T) + 15) / 16 * 16 : 0;
   WorkspaceHold hold;
@@ -1168,7 +1174,8 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
 
   a.dev = dev;
   const bool wide = N * a.G > 16 * R;   // some request has more than one tile of 16 columns
-  const int64_t steps = (M * c.page + kStep - 1) / kStep;
+  // steps of a tile, at most
+  const int64_t all = (M * c.page + kStep - 1) / kStep, seen = ((int64_t)a.reach + kStep - 1) / kStep + 1, steps = all < seen ? all : seen;
 #define KV_ATTENTION(T) return format == RAI_KV_E4M3 ? launch_by_features<T, RAI_KV_E4M3>(st, a, odd, wide, steps) : launch_by_features<T, RAI_KV_INT8>(st, a, odd, wide, steps)
   if (q->dtype == RAI_BF16) KV_ATTENTION(bf16_raw);
   if (q->dtype == RAI_F16) KV_ATTENTION(f16_raw);
