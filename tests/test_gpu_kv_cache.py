@@ -390,6 +390,98 @@ def test_attention_is_the_same_every_time_and_beside_other_threads(hip):
     assert not failed
 
 
+@pytest.mark.parametrize("dt,heads,kv,dim,window", [("bf16", 12, 2, 128, 0), ("f16", 8, 1, 64, 0), ("f32", 8, 2, 80, 0), ("bf16", 6, 1, 256, 0), ("f32", 4, 1, 256, 700), ("bf16", 12, 2, 128, 1900)])
+def test_attention_of_few_and_many_columns_over_long_contexts(hip, dt, heads, kv, dim, window):
+    """Both kinds of tiles in one launch, whole ones and ones that workers share, and requests of neither."""
+    rng = np.random.default_rng(dim + heads)
+    for page, form, total, new in ((16, "e4m3", [6000, 3000, 700, 5000, 1, 0], [1, 200, 1, 65, 1, 0]), (128, "int8", [2500, 4100, 4100], [300, 1, 2])):
+        b = Batch(rng, total, new, page, kv, dim, form)
+        check_attention(b, rows(rng, (b.N, heads, dim), dt), dt, heads, window)
+
+
+@pytest.mark.parametrize("dt,dim", [("bf16", 64), ("f16", 80), ("f32", 128), ("bf16", 256)])
+def test_attention_of_long_contexts_over_many_heads(hip, dt, dim):
+    """Few workers to a head: the last of them to leave a tile joins its parts.  Twice, since it also sets its count back."""
+    rng = np.random.default_rng(dim)
+    for new in ([1, 1, 1], [1, 30, 1]):
+        b = Batch(rng, [5000, 2900, 170], new, 64, 20, dim, "e4m3")
+        q = rows(rng, (b.N, 20, dim), dt)
+        for _ in range(2):
+            check_attention(b, q, dt, 20)
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_attention_of_more_requests_than_a_wave_has_lanes(hip, new):
+    rng = np.random.default_rng(31 + new)
+    total = [int(rng.integers(new, 2600 if i % 40 == 0 else 60)) for i in range(200)]
+    b = Batch(rng, total, [new if i % 3 else 0 for i in range(200)], 16, 2, 64, "int8")
+    check_attention(b, rows(rng, (b.N, 8, 64), "bf16"), "bf16", 8)
+
+
+def test_attention_of_tables_that_are_part_of_wider_ones(hip):
+    rng = np.random.default_rng(32)
+    b = Batch(rng, [700, 90], [1, 40], 16, 2, 64, "e4m3")
+    wide = rng.integers(0, 2 ** 32, (2, b.M + 11), dtype=np.uint32)
+    wide[:, 3:3 + b.M] = b.tables
+    q = rows(rng, (b.N, 8, 64), "bf16")
+    got = down(b.cache().attention(up(q, "bf16"), dev(wide, "u32").narrow(1, 3, b.M), dev(b.starts, "i64"), dev(b.lens, "i64"), 0.125)).astype(np.float64)
+    want, spread, slip = O.attention(q, b.tables, b.starts, b.lens, b.form, b.k, b.v, b.k_scale, b.v_scale, 16, 0.125)
+    assert (np.abs(got - want) <= attention_bound(want, spread, slip, "bf16", 64, 700)).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+def test_attention_does_not_see_what_others_left(hip, dim, dt):
+    """Registers, LDS, scratch and freed memory full of NaN from the calls before: results are those of a first call, bit for bit."""
+    rng = np.random.default_rng(33)
+    bad = ops.full(float("nan"), (4, 12, 256, 128), "bf16")
+    for total, new in (([70, 150], [1, 1]), ([40, 90], [21, 5]), ([4000, 900], [1, 70])):
+        b = Batch(rng, total, new, 32, 1, dim, "e4m3")
+        c, q = b.cache(), up(rows(rng, (b.N, 8, dim), dt), dt)
+        rest = (dev(b.tables, "u32"), dev(b.starts, "i64"), dev(b.lens, "i64"), dim ** -0.5)
+        first = c.attention(q, *rest).to_storage()
+        nan = up(np.full((b.N, 8, dim), np.nan, np.float32), dt)
+        for _ in range(5):
+            ops.attention(bad, bad, bad, 0.1, 1, 0)
+            c.attention(nan, *rest)
+            held = [ops.full(float("nan"), (n,), "f32") for n in (64, 1024, 16384, 1 << 20)]
+            del held
+            assert np.array_equal(c.attention(q, *rest).to_storage(), first)
+
+
+def test_caches_of_more_than_two_to_the_32_bytes(hip):
+    """Pages whose codes lie behind 2^32 bytes: rows appended to them, and read back by attention of few columns and of many."""
+    from rai_amd.kv_cache import KvCache
+
+    rng = np.random.default_rng(34)
+    pages, heads, dim, page = 70000, 2, 256, 128   # 4.6 GB of keys and as much of values
+    cache = KvCache(pages, heads, dim, page, "e4m3")
+    far = [65537, 69999, 0, 65535, 65536]
+    total = [300, 200]
+    tables = np.array([far[:3], far[3:] + [1]], np.uint32)
+    k, v = (rows(rng, (500, heads, dim), "bf16") for _ in range(2))
+    runs = np.array([(far[0], 0, 0, 128), (far[1], 0, 128, 128), (far[2], 0, 256, 44), (far[3], 0, 300, 128), (far[4], 0, 428, 72)], np.uint32).T
+    ops.index_errors()
+    cache.append(up(k, "bf16"), up(v, "bf16"), dev(runs, "u32"))
+    small = [t.narrow(0, 0, 2).to_storage()[[0] * 3 + [1] * 3] * 0 for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    for i, p in enumerate(far):
+        for mine, t in zip(small, (cache.k, cache.v, cache.k_scale, cache.v_scale)):
+            mine[i] = t.narrow(0, p, 1).to_storage()[0]
+    near = np.array([(i, r[1], r[2], r[3]) for i, r in enumerate(runs.T)], np.uint32).T
+    for rows_, at, transposed in ((k, 0, False), (v, 1, True)):
+        codes, scale, refused = O.append(rows_, near, "e4m3", small[at] * 0, small[2 + at] * 0, transposed)
+        same(small[at], codes, "codes")
+        same(small[2 + at], scale, "scales")
+    table_near = np.array([[0, 1, 2], [3, 4, 5]], np.uint32)
+    for new in ([1, 1], [40, 3]):
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
+        q = rows(rng, (sum(new), 4, dim), "bf16")
+        got = down(cache.attention(up(q, "bf16"), dev(tables, "u32"), dev(starts, "i64"), dev(np.array(total, np.int64), "i64"), 0.0625)).astype(np.float64)
+        want, spread, slip = O.attention(q, table_near, starts, np.array(total), "e4m3", *small, page, 0.0625)
+        assert (np.abs(got - want) <= attention_bound(want, spread, slip, "bf16", dim, 300)).all()
+    assert ops.index_errors() == 0
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("form,inter", [("e4m3", False), ("int8", True)])
 def test_steps_of_a_serving_loop(hip, form, inter):
