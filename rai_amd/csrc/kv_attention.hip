@@ -120,6 +120,11 @@ constexpr int kv_blocks(int vt, int nc, int terms) { return vt > 8 || (nc > 1 &&
 // 2048 over 32 heads (not full) 19 against 14, and 16 of up to 4000 (63, full) 40 against 38; of many, a window of 512 keys (10) 38 against 42, 16 chunks of up
 // to 256 behind up to 700 (11) 28 against 43, 8 of up to 1024 with nothing before (16) 56 against 62, but a window of 1024 (18) 57 against 51.
 constexpr int kv_alone(int nc, bool full) { return nc ? 16 : full ? 40 : 24; }
+// Requests of many columns go through tiles of few as well where all tiles of 16 find room on the card at once and have up to so many steps for each place there: four
+// waves then share a tile's steps, and no tile waits for another.  So against tiles of many: 9 chunks of up to 37 in a window of 512 keys (f32, 256 features, 4 steps a
+// place) 29 us against 38, 640 rows behind nothing (10) 17 against 24, 4 chunks of up to 64 behind up to 4000 (15) 26 against 47, 16 of up to 64 behind
+// up to 2000 (f32, 28) 36 against 43; beyond, 300 rows behind 5000 (35) 50 against 43, 16 chunks of up to 64 behind up to 4000 (56) 49 against 43.
+constexpr int kv_small = 32;
 // Steps of a share at least.
 constexpr int kv_least(int nc) { return nc ? 2 : 8; }
 // Workers of a key head up to which the last one to leave a tile joins its parts.
@@ -1047,6 +1052,8 @@ template <typename T, int VT, int NC> struct KvShares {
 
 template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_t st, KvAttnArgs a, const KvRowsArgs &odd, bool wide, int64_t steps) {
   constexpr int NC = wide_tiles<T>(16 * VT);
+  const int64_t tiles = (a.N * a.G / 16 + a.R) * a.Hkv, slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, 1, KvTerms<T>::n);
+  if (tiles <= slots && tiles * steps <= kv_small * slots) wide = false;
   const KvShares<T, VT, 0> few(a, steps, wide ? a.R : a.N * a.G / 16 + a.R);
   const KvShares<T, VT, NC> many(a, steps, a.N * a.G / (32 * NC) + a.R);
   const size_t of_few = few.bytes(a), of_many = wide ? many.bytes(a) : 0;

@@ -399,6 +399,37 @@ def test_attention_of_few_and_many_columns_over_long_contexts(hip, dt, heads, kv
         check_attention(b, rows(rng, (b.N, heads, dim), dt), dt, heads, window)
 
 
+@pytest.mark.parametrize("longest", [500, 1500])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [16, 64, 72, 80, 100, 128, 192, 256])
+def test_attention_of_many_columns(hip, dim, dt, longest):
+    """More rows than tiles of few columns hold at once: tiles of many, whole ones and (of long contexts) ones that workers share."""
+    rng = np.random.default_rng(dim + longest)
+    b = Batch(rng, [longest, 90, 257, 40], [199, 60, 57, 1], 32, 2, dim, "e4m3" if dim % 3 else "int8")
+    check_attention(b, rows(rng, (b.N, 40, dim), dt), dt, 40)
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("window", [1, 63, 100, 1000])
+def test_attention_of_many_columns_in_windows(hip, page, window):
+    rng = np.random.default_rng(page + window)
+    for dt, form, heads, kv in (("bf16", "e4m3", 40, 1), ("f32", "int8", 41, 1)):
+        b = Batch(rng, [1400, 33, 300, 64], [250, 33, 40, 2], page, kv, 64, form)
+        check_attention(b, rows(rng, (b.N, heads, 64), dt), dt, heads, window)
+
+
+def test_attention_of_many_columns_with_a_scale_below_zero_and_missing_pages(hip):
+    rng = np.random.default_rng(35)
+    b = Batch(rng, [300, 200], [280, 60], 16, 1, 64, "e4m3")
+    q = rows(rng, (b.N, 40, 64), "bf16")
+    for scale in (20.0, -3.0, 0.0):
+        check_attention(b, q, "bf16", 40, scale=scale)
+    b.tables[0, 2], b.tables[1, 5], b.tables[1, 6] = b.pages, 2 ** 32 - 1, b.pages + 3
+    ops.index_errors()
+    check_attention(b, q, "bf16", 40)
+    assert ops.index_errors() > 0
+
+
 @pytest.mark.parametrize("dt,dim", [("bf16", 64), ("f16", 80), ("f32", 128), ("bf16", 256)])
 def test_attention_of_long_contexts_over_many_heads(hip, dt, dim):
     """Few workers to a head: the last of them to leave a tile joins its parts.  Twice, since it also sets its count back."""
