@@ -76,11 +76,14 @@ template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, u
 // Read by one tile alone, so not to be kept in the L2.
 __device__ __forceinline__ kv_u32x4 fetch_once(const uint8_t *p) { return __builtin_nontemporal_load(reinterpret_cast<const kv_u32x4 *>(p)); }
 
-// How many bf16 hold a value of type T: products with codes are then exact, so f16 and f32 rows lose nothing on the bf16 matrix instructions.
+// How many bf16 hold a value of type T: products with codes are then exact, so f16 and f32 rows lose nothing on the bf16 matrix instructions.  The softmax's
+// weights are rounded to as many, of tiles of few columns to two at least: with one, results of bf16 rows are off by 0.0022 to 0.0024 of their size, with two by 0.0016
+// to 0.0017, which is the output's own rounding, and a step that waits for memory has room for it (64 requests 53 us either way).  Tiles of many
+// columns, bound by instructions, keep one (prompts of 2300 rows 85 us, with two 100).
 template <typename T> struct KvTerms;
-template <> struct KvTerms<bf16_raw> { static constexpr int n = 1; };
-template <> struct KvTerms<f16_raw> { static constexpr int n = 2; };
-template <> struct KvTerms<float> { static constexpr int n = 3; };
+template <> struct KvTerms<bf16_raw> { static constexpr int n = 1, weights = 2; };
+template <> struct KvTerms<f16_raw> { static constexpr int n = 2, weights = 2; };
+template <> struct KvTerms<float> { static constexpr int n = 3, weights = 3; };
 
 __device__ __forceinline__ float bf16_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // Two values' terms: cut off (not rounded), so that what is left is exact, the last term rounded.
@@ -548,7 +551,7 @@ __device__ __forceinline__ void kv_meet() {
 template <typename T, int VT> constexpr int kv_few_lds() { return 4 * VT * 64 * 16 + 4 * 2 * 64 * 4; }
 template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
   typedef KvFeatures<VT> Fe;
-  constexpr int TERMS = KvTerms<T>::n, QT = 16, KS = Fe::KS, KN = Fe::KN, KW = 4;
+  constexpr int TERMS = KvTerms<T>::n, WEIGHTS = KvTerms<T>::weights, QT = 16, KS = Fe::KS, KN = Fe::KN, KW = 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
@@ -653,15 +656,15 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
           }
         }
         load_keys(next, of_k);
-        kv_bf16x8 pf[1][2][TERMS];
-        kv_weights<VT, 1, TERMS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone), pf);
+        kv_bf16x8 pf[1][2][WEIGHTS];
+        kv_weights<VT, 1, WEIGHTS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_first || st * kStep < lo_last || __any(gone), pf);
 #pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const kv_bf16x8 f = kv_unpack<FMT>(now.v[t][2 * u], now.v[t][2 * u + 1]);
 #pragma unroll
-            for (int i = 0; i < TERMS; ++i) z.o[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[0][u][i], z.o[0][t], 0, 0, 0);
+            for (int i = 0; i < WEIGHTS; ++i) z.o[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[0][u][i], z.o[0][t], 0, 0, 0);
           }
         load_values(next, of_v);
         next = ahead;
@@ -716,7 +719,7 @@ __device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
 template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
   typedef KvFeatures<VT> Fe;
-  constexpr int TERMS = KvTerms<T>::n, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
+  constexpr int TERMS = KvTerms<T>::n, WEIGHTS = TERMS, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w >> 1;
   const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
@@ -862,8 +865,8 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
                 for (int i = 0; i < TERMS; ++i) s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[c][e][i], s[c][t], 0, 0, 0);
             }
           }
-          kv_bf16x8 pf[NC][2][TERMS];
-          kv_weights<VT, NC, TERMS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_near || st * kStep < lo_near || __any(gone), pf);
+          kv_bf16x8 pf[NC][2][WEIGHTS];
+          kv_weights<VT, NC, WEIGHTS>(s, z, cols, scales, a.scale_log2, key0, (st + 1) * kStep - 1 > hi_near || st * kStep < lo_near || __any(gone), pf);
 #pragma unroll
           for (int t = 0; t < VT; ++t) {
             const kv_u32x4 v = *reinterpret_cast<const kv_u32x4 *>(vt + (g * 16 * VT + 16 * t + col) * 16);
@@ -873,7 +876,7 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
 #pragma unroll
               for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i) z.o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], z.o[c][t], 0, 0, 0);
+                for (int i = 0; i < WEIGHTS; ++i) z.o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pf[c][u][i], z.o[c][t], 0, 0, 0);
             }
           }
         }
