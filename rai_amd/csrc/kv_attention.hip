@@ -18,7 +18,6 @@ struct KvKind {
   int workers;                   // of a key head, each with an even share of the steps; 0: a worker to a tile
   int each, extra;               // sixteenths of a key that a tile sees more than the one before it, and that its beginning and end are worth
   int least;                     // steps of a share at least
-  int count;                     // whether the block that leaves a tile's last part joins the parts, or another launch
   double per_worker;             // 1 / workers
   float *part;                   // [Hkv * workers][2][columns of a tile][features] sums of a share's first and last tile
   float *part_m, *part_l;        // their maxima and sums of weights
@@ -48,11 +47,6 @@ struct KvAttnArgs {
   unsigned long long *errors;
   KvKind few, many;
 };
-
-// Counts of the workers that have left their part of a tile; the one that counts itself in last joins the parts and sets the count back to
-// zero.  By the first part's place: two to a worker.  Shared by all launches on a device, which run one after the other.
-constexpr int kKvTickets = 1 << 17;
-__device__ int kv_tickets[kKvTickets];
 
 // Eight codes as the eight bf16 of a fragment: every e4m3 value and every whole number up to 127 is a bf16.
 template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, uint32_t hi) {
@@ -128,12 +122,12 @@ constexpr int kv_alone(int nc, bool full) { return nc ? 16 : full ? 40 : 24; }
 // place) 29 us against 38, 640 rows behind nothing (10) 17 against 24, 4 chunks of up to 64 behind up to 4000 (15) 26 against 47, 16 of up to 64 behind
 // up to 2000 (f32, 28) 36 against 43; beyond, 300 rows behind 5000 (35) 50 against 43, 16 chunks of up to 64 behind up to 4000 (56) 49 against 43.
 constexpr int kv_small = 32;
-// Steps of a share at least.
+// Steps of a share at least.  Of few columns with 8, with 4 and with 16: one request of 100000 keys 30, 47 and 23 us, of 8000 15, 13 and 19, four of 4000 over 8 heads 17, 19 and 22;
+// of many with 2, 1 and 4: 700 rows behind 8000 keys 75, 76 and 77.
 constexpr int kv_least(int nc) { return nc ? 2 : 8; }
-// Workers of a key head up to which the last one to leave a tile joins its parts.
-constexpr int kv_counted = 32;
-// Steps that a tile's beginning and end take as long as.
-constexpr int kv_extra(int nc) { return nc ? 6 : 12; }
+// Steps that a tile's beginning and end take as long as.  Prompts of 2300 rows 105 us with 3, 100 with 6, 105 with 9, 110 with 12; one request of 8000 keys 14.5 us
+// with 6, 19 with 12.
+constexpr int kv_extra = 6;
 
 // How the work of a key head is dealt out.  A tile of a request is as long as the keys that its last row sees, which grows evenly from tile to
 // tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1), and `extra` for its beginning and end
@@ -217,7 +211,7 @@ template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, c
       if (d.workers) {
         out->share = max((int64_t)((double)total * d.per_worker) + 1, (int64_t)d.least * kUnits);   // times the workers: no less than the total
         u = worker * out->share;
-        if (!d.count && threadIdx.x == 0) d.join[(int64_t)kvh * d.workers + worker].first = -1;
+        if (threadIdx.x == 0) d.join[(int64_t)kvh * d.workers + worker].first = -1;
       }
       if (u >= total) return false;
     }
@@ -437,28 +431,12 @@ __device__ __forceinline__ void kv_weights(kv_f32x4 (&s)[NC][4], KvState<VT, NC>
     }
   }
 }
-// The L2s of the XCDs are not coherent for ordinary accesses: what blocks hand to one another is written through and read around them.
-__device__ __forceinline__ void kv_put(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float kv_get(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void kv_put4(float *p, kv_f32x4 v) {
-  struct Pair { uint64_t a, b; } x = __builtin_bit_cast(Pair, v);
-  __hip_atomic_store((uint64_t *)p, x.a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __hip_atomic_store((uint64_t *)p + 1, x.b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ kv_f32x4 kv_get4(const float *p) {
-  struct Pair { uint64_t a, b; } x;
-  x.a = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  x.b = __hip_atomic_load((const uint64_t *)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return __builtin_bit_cast(kv_f32x4, x);
-}
-
 // The end of a tile, or of a worker's part of one.  The wave holds columns c0 .. of the tile and of their features the tiles t0, t0 + step, ..; held:
-// whether it holds any.  A whole tile goes to the output, a part to the scratch, from where another launch joins them; or (COUNT, d.count)
-// each part is counted in, and the block that counts itself in last, which waits for nobody, joins them and writes the output.  That saves the
-// launch, but reads one part after the other: it serves where a tile has few workers.
-template <typename T, bool COUNT, int OT, int NC>
+// whether it holds any.  A whole tile goes to the output, a part to the scratch, from where another launch joins them.  (Parts joined by the last
+// block to leave a tile, without that launch, took as long or longer: 16 requests of up to 8000 keys over 16 heads 37 us for 34.)
+template <typename T, int OT, int NC>
 __device__ __forceinline__ void kv_finish(const KvAttnArgs &a, const KvKind &d, const KvWork &k, int kvh, int worker, bool first, int64_t size, int64_t to, int QT, int c0, int t0, int step,
-                                          bool held, const KvColumns<NC> &cols, KvState<OT, NC> &z, int *sh_last) {
+                                          bool held, const KvColumns<NC> &cols, const KvState<OT, NC> &z) {
   const int col = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
   auto feature = [&](int i) { return 16 * (t0 + step * i) + 4 * g; };
   if (k.from != 0 || to != size) {
@@ -475,44 +453,15 @@ __device__ __forceinline__ void kv_finish(const KvAttnArgs &a, const KvKind &d, 
       if (!cols.live[c] || !held) continue;
       const int64_t e = row_of(2 * own + !first, c);
       if (g == 0 && t0 == 0) {
-        kv_put(d.part_m + e, z.m[c]);
-        kv_put(d.part_l + e, z.l[c]);
+        d.part_m[e] = z.m[c];
+        d.part_l[e] = z.l[c];
       }
 #pragma unroll
       for (int i = 0; i < OT; ++i)
-        if (feature(i) < a.features) {
-          float *const p = d.part + e * a.features + feature(i);
-          if (COUNT && d.count) kv_put4(p, z.o[c][i]);
-          else *reinterpret_cast<kv_f32x4 *>(p) = z.o[c][i];
-        }
+        if (feature(i) < a.features) *reinterpret_cast<kv_f32x4 *>(d.part + e * a.features + feature(i)) = z.o[c][i];
     }
-    if (!COUNT || !d.count) {
-      if (to == size && threadIdx.x == 0) d.join[own] = KvJoin{(int)begin, (int)place, k.req.start, k.tile * QT, min(QT, k.req.n * a.G - k.tile * QT)};
-      return;
-    }
-    const int64_t end = worker_of(k.tile_at + size - 1);
-    int *const ticket = kv_tickets + 2 * ((int64_t)kvh * d.workers + begin) + place;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this thread has written through is there
-    __syncthreads();
-    if (threadIdx.x == 0) *sh_last = atomicAdd(ticket, 1) == end - begin;
-    __syncthreads();
-    const bool last = *sh_last;
-    if (!last) return;
-    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    z.clear();
-    for (int64_t w = begin; w <= end; ++w) {
-      const int64_t at = 2 * ((int64_t)kvh * d.workers + w) + (w == begin ? place : 0);
-      KvState<OT, NC> y;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int64_t e = cols.live[c] ? row_of(at, c) : at * QT;   // (a column that is not there reads the tile's first)
-        y.m[c] = kv_get(d.part_m + e);
-        y.l[c] = kv_get(d.part_l + e);
-#pragma unroll
-        for (int i = 0; i < OT; ++i) y.o[c][i] = kv_get4(d.part + e * a.features + (feature(i) < a.features ? feature(i) : 0));
-      }
-      z.add(y);
-    }
+    if (to == size && threadIdx.x == 0) d.join[own] = KvJoin{(int)begin, (int)place, k.req.start, k.tile * QT, min(QT, k.req.n * a.G - k.tile * QT)};
+    return;
   }
   if (!held) return;
 #pragma unroll
@@ -548,8 +497,11 @@ __device__ __forceinline__ void kv_meet() {
 // the scores of sixteen neighbouring keys, which are the 16 bytes that it loads of a feature of V: the weights are the second product's
 // fragments as they lie in registers, and every load of the cache is 16 bytes a lane, straight to registers.  Sixteen keys lie in one
 // page, so a lane group has one page and one scale of keys and of values.
+// Bound by memory and by what comes before the first step and behind the last: 64 requests of up to 16384 keys (236 MB) take 47 us and their join 4.7, 4.6 TB/s
+// in all where a read alone reaches 7.1 and a copy 4.7; a lone row over 777 keys takes 10 us, a chain of trips (lengths, table, keys, merge) and of code that is
+// run once.  A quarter of a wave reads sixteen keys' 16 bytes at a time: read as whole lines, at other results, the large case took 50 us.
 template <typename T, int VT> constexpr int kv_few_lds() { return 4 * VT * 64 * 16 + 4 * 2 * 64 * 4; }
-template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
+template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
   typedef KvFeatures<VT> Fe;
   constexpr int TERMS = KvTerms<T>::n, WEIGHTS = KvTerms<T>::weights, QT = 16, KS = Fe::KS, KN = Fe::KN, KW = 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -701,7 +653,7 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
 #pragma unroll
       for (int t = 0; t < OT; ++t) y.o[0][t] += sums[i][min(4 * t + w, VT - 1)][lane] * f[i];
     }
-    kv_finish<T, true, OT, 1>(a, d, k, kvh, worker, first, size, to, QT, 0, w, 4, true, cols, y, sh_last);
+    kv_finish<T, OT, 1>(a, d, k, kvh, worker, first, size, to, QT, 0, w, 4, true, cols, y);
     if (!kv_next<QT>(a, d, size, to, &k)) return;
   }
 }
@@ -716,8 +668,11 @@ __device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
 // through LDS as codes, two buffers of two steps, one barrier for both: each byte of the cache reaches a CU once for 32 NC columns, and no
 // register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
 // rows, their 16-byte pieces exchanged so that sixteen rows' reads spread over the banks; values as sixteen keys of a feature.
+// Bound by the instructions around the products: a step of 32 columns takes 64 matrix instructions (1024 clocks of a SIMD) and about 300 vector ones
+// (1600: codes to bf16 128, the softmax 160) and as many scalar ones in between, two waves to a SIMD.  Prompts of 2300 rows over up to 5000 keys, 34.6 GFLOP, take 77 us and
+// their joins 8 and 5; sixteen of them 225 us, 530 TFLOP/s of the 1370 that a large product reaches.  Of the 77, 13 are workers' first and last trips.
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
-template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds, int *sh_last) {
+template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
   typedef KvFeatures<VT> Fe;
   constexpr int TERMS = KvTerms<T>::n, WEIGHTS = TERMS, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w >> 1;
@@ -916,7 +871,7 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
       }
       z.add(y);
     }
-    kv_finish<T, false, VT, NC>(a, d, k, kvh, worker, first, size, to, QT, (w & 1) * 16 * NC, 0, 1, half == 0, cols, z, sh_last);
+    kv_finish<T, VT, NC>(a, d, k, kvh, worker, first, size, to, QT, (w & 1) * 16 * NC, 0, 1, half == 0, cols, z);
     if (!kv_next<QT>(a, d, size, to, &k)) return;
   }
 }
@@ -926,18 +881,17 @@ template <typename T, int FMT, int VT, int NC>
 __global__ void __launch_bounds__(256, kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n)) k_kv_attention(KvAttnArgs a) {
   constexpr int FEW = kv_few_lds<T, VT>(), WIDE = NC ? kv_wide_lds<VT>() : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[FEW > WIDE ? FEW : WIDE];
-  __shared__ int sh_last;
   if constexpr (NC > 0) {
     if ((int)blockIdx.x < a.many.blocks) {
-      kv_wide<T, FMT, VT, NC>(a, a.many, blockIdx.x, lds, &sh_last);
+      kv_wide<T, FMT, VT, NC>(a, a.many, blockIdx.x, lds);
       return;
     }
   }
-  kv_few<T, FMT, VT>(a, a.few, blockIdx.x - (NC ? a.many.blocks : 0), lds, &sh_last);
+  kv_few<T, FMT, VT>(a, a.few, blockIdx.x - (NC ? a.many.blocks : 0), lds);
 }
 
 // The parts of tiles that workers share, to the output.  Blocks for each worker that had a tile's last part, over the tile's columns: a wave reads whole rows of
-// as many columns as fit it.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
+// as many columns as fit it.  4.7 us behind 64 requests, 8 behind prompts of 2300 rows, most of it the launch and one trip.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
 template <typename T, bool PARTS> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, KvKind d, int QT) {
   __shared__ kv_f32x4 sums[4][64];
   __shared__ float stats[4][2][64];
@@ -1028,7 +982,7 @@ template <typename T, int VT, int NC> struct KvShares {
   int64_t parts;
   // tiles: as many as there may be.  No more workers than the least share allows: blocks that find nothing to do take their time too.
   KvShares(const KvAttnArgs &a, int64_t steps, int64_t tiles) {
-    const int64_t slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n) / a.Hkv, useful = (tiles * (steps + kv_extra(NC)) + kv_least(NC) - 1) / kv_least(NC);
+    const int64_t slots = (int64_t)device_cu_count(a.dev) * kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n) / a.Hkv, useful = (tiles * (steps + kv_extra) + kv_least(NC) - 1) / kv_least(NC);
     const int64_t n = slots < useful ? slots : useful;
     workers = steps <= kv_alone(NC, 2 * tiles >= slots) ? 0 : n < 1 ? 1 : (int)n;
     parts = 2ll * QT * a.Hkv * workers;
@@ -1041,9 +995,8 @@ template <typename T, int VT, int NC> struct KvShares {
     d.workers = workers;
     d.blocks = (workers ? workers : (int)(which == 1 ? a.R : a.N * a.G / QT + a.R)) * a.Hkv;
     d.each = (16 * QT + a.G - 1) / a.G;
-    d.extra = kv_extra(NC) * kUnits;
+    d.extra = kv_extra * kUnits;
     d.least = kv_least(NC);
-    d.count = NC == 0 && workers <= kv_counted && 2 * a.Hkv * workers <= kKvTickets;
     d.per_worker = workers ? 1.0 / workers : 0;
     d.part = (float *)ws;
     d.part_m = d.part + parts * a.features;
@@ -1089,7 +1042,7 @@ template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_
   }
   RAI_TRY(launch_check("kv_attention"));
   const int per_wave = 256 / a.features;
-  if (a.few.workers && !a.few.count) {
+  if (a.few.workers) {
     hipLaunchKernelGGL((k_kv_attention_join<T, true>), dim3((unsigned)a.few.workers, (unsigned)a.Hkv, (unsigned)((few.QT + per_wave - 1) / per_wave)), dim3(256), 0, st, a, a.few, few.QT);
     RAI_TRY(launch_check("kv_attention_join"));
   }
