@@ -400,11 +400,11 @@ int rai_hip_kv_append(int dev, const rai_hip_tensor *new_k, const rai_hip_tensor
  * [N, Hq, D] contiguous in q's dtype; rows that belong to no request are left as they are.
  *   tables u32 [R, M] (unit stride along M), starts i64 [R + 1] not falling, lens i64 [R] (after rai_hip_kv_plan: out_lens)
  * Pages of a shared prefix may stand in many tables.  A page number that is not there hides its tokens, and counts as an index error, as
- * does a length past M * page, of which the first M * page tokens are seen.  Scales are positive (a page whose scale is not counts as one of
- * scale 1 for its values); codes that are NaN (no rai_hip_kv_append writes one) may reach rows that do not see their token.  Products are exact
- * and summed in f32; weights are rounded to 16 bits or more of which bf16 rows of large batches (more than 16 rows of a head to a block's
- * place on the device) keep 8.  Long contexts are cut over blocks: their sums go through the device's scratch, of a size that
- * does not grow with the batch, as do rows off 16-byte boundaries and heads of features in no whole eights, of a size that does. */
+ * does a length past M * page, of which the first M * page tokens are seen.  Scales are positive.  Codes that are NaN (no
+ * rai_hip_kv_append writes one) may reach rows that do not see their token.  Products are exact and sums in f32; weights are rounded to 16
+ * significant bits or more, to 8 for bf16 rows of batches that fill the device many times over.  Long contexts are cut over blocks: their sums go
+ * through the device's scratch, of a size that does not grow with the batch, as do rows off 16-byte boundaries and heads whose
+ * features are in no whole eights, of one that does. */
 int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_hip_tensor *tables, const rai_hip_tensor *starts, const rai_hip_tensor *lens,
                          int32_t format, const rai_hip_tensor *k, const rai_hip_tensor *v, const rai_hip_tensor *k_scale,
                          const rai_hip_tensor *v_scale, double scale, int32_t window, const rai_hip_tensor *out);

@@ -670,7 +670,7 @@ __device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
 // rows, their 16-byte pieces exchanged so that sixteen rows' reads spread over the banks; values as sixteen keys of a feature.
 // Bound by the instructions around the products: a step of 32 columns takes 64 matrix instructions (1024 clocks of a SIMD) and about 300 vector ones
 // (1600: codes to bf16 128, the softmax 160) and as many scalar ones in between, two waves to a SIMD.  Prompts of 2300 rows over up to 5000 keys, 34.6 GFLOP, take 77 us and
-// their joins 8 and 5; sixteen of them 225 us, 530 TFLOP/s of the 1370 that a large product reaches.  Of the 77, 13 are workers' first and last trips.
+// their join 9; sixteen of them 225 us, 530 TFLOP/s of the 1370 that a large product reaches.  Of the 77, 13 are workers' first and last trips.
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
 template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
   typedef KvFeatures<VT> Fe;
@@ -891,17 +891,14 @@ __global__ void __launch_bounds__(256, kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n)
 }
 
 // The parts of tiles that workers share, to the output.  Blocks for each worker that had a tile's last part, over the tile's columns: a wave reads whole rows of
-// as many columns as fit it.  4.7 us behind 64 requests, 8 behind prompts of 2300 rows, most of it the launch and one trip.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
-template <typename T, bool PARTS> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, KvKind d, int QT) {
-  __shared__ kv_f32x4 sums[4][64];
-  __shared__ float stats[4][2][64];
-  const int worker = blockIdx.x, kvh = blockIdx.y;
+// as many columns as fit it.  4.7 us behind 64 requests, 9 behind prompts of 2300 rows, most of it the launch and one trip.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
+template <typename T, bool PARTS> __device__ __forceinline__ void kv_join(const KvAttnArgs &a, const KvKind &d, int QT, int worker, int kvh, int z, kv_f32x4 (*sums)[64], float (*stats)[2][64]) {
   const int64_t base = (int64_t)kvh * d.workers;
   const KvJoin j = d.join[base + worker];
   const int F4 = a.features / 4, per_wave = 64 / F4, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = (PARTS ? blockIdx.z : blockIdx.z * 4 + w) * per_wave + lane / F4, f = lane % F4 * 4;
+  const int c = (PARTS ? z : z * 4 + w) * per_wave + lane / F4, f = lane % F4 * 4;
   const bool live = j.first >= 0 && lane / F4 < per_wave && c < j.columns;
-  if (j.first < 0 || (PARTS && (int)blockIdx.z * per_wave >= j.columns)) return;
+  if (j.first < 0 || (PARTS && z * per_wave >= j.columns)) return;
   const int cc = live ? c : 0;
   float m = kNoScore, l = 0.f;
   kv_f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -943,6 +940,25 @@ template <typename T, bool PARTS> __global__ void __launch_bounds__(256) k_kv_at
 #pragma unroll
   for (int u = 0; u < 4; ++u) Scalar<T>::store(&y.v[u], l == 0.f ? 0.f : o[u] * over);
   *reinterpret_cast<Four *>((T *)a.out + (((int64_t)j.start + i) * a.Hq + (int64_t)kvh * a.G + x - i * a.G) * a.D + f) = y;
+}
+
+// Of few columns alone, a grid of workers, heads and columns; or of both kinds, `few` blocks, zf to a worker, then those of many columns, zm to a worker.  (One launch for
+// both: a chunk of 64 rows behind 30000 keys 51 us, with two 61; but found from one number, a block's place costs the few alone 1.7 us.)
+template <typename T, bool BOTH> __global__ void __launch_bounds__(256) k_kv_attention_join(KvAttnArgs a, int few, int zf, int zm, int QT) {
+  __shared__ kv_f32x4 sums[4][64];
+  __shared__ float stats[4][2][64];
+  if constexpr (!BOTH) kv_join<T, true>(a, a.few, 16, blockIdx.x, blockIdx.y, blockIdx.z, sums, stats);
+  else {
+    int b = blockIdx.x;
+    if (b < few) {
+      const int z = b % zf, own = b / zf;
+      kv_join<T, true>(a, a.few, 16, own % a.few.workers, own / a.few.workers, z, sums, stats);
+    } else {
+      b -= few;
+      const int z = b % zm, own = b / zm;
+      kv_join<T, false>(a, a.many, QT, own % a.many.workers, own / a.many.workers, z, sums, stats);
+    }
+  }
 }
 
 // Tiles of 16 columns to a wave of a wide block: as many as registers hold.
@@ -1041,16 +1057,11 @@ template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_
     hipLaunchKernelGGL((k_kv_attention<T, FMT, VT, 0>), grid, dim3(256), 0, st, a);
   }
   RAI_TRY(launch_check("kv_attention"));
-  const int per_wave = 256 / a.features;
-  if (a.few.workers) {
-    hipLaunchKernelGGL((k_kv_attention_join<T, true>), dim3((unsigned)a.few.workers, (unsigned)a.Hkv, (unsigned)((few.QT + per_wave - 1) / per_wave)), dim3(256), 0, st, a, a.few, few.QT);
-    RAI_TRY(launch_check("kv_attention_join"));
-  }
-  if (a.many.workers) {
-    hipLaunchKernelGGL((k_kv_attention_join<T, false>), dim3((unsigned)a.many.workers, (unsigned)a.Hkv, (unsigned)((many.QT + 4 * per_wave - 1) / (4 * per_wave))), dim3(256), 0, st, a,
-                       a.many, many.QT);
-    RAI_TRY(launch_check("kv_attention_join"));
-  }
+  const int per_wave = 256 / a.features, zf = (few.QT + per_wave - 1) / per_wave, zm = (many.QT + 4 * per_wave - 1) / (4 * per_wave);
+  const int64_t of_few_tiles = (int64_t)a.few.workers * a.Hkv * zf, joins = of_few_tiles + (int64_t)a.many.workers * a.Hkv * zm;
+  if (a.many.workers) hipLaunchKernelGGL((k_kv_attention_join<T, true>), dim3((unsigned)joins), dim3(256), 0, st, a, (int)of_few_tiles, zf, zm, many.QT);
+  else if (a.few.workers) hipLaunchKernelGGL((k_kv_attention_join<T, false>), dim3((unsigned)a.few.workers, (unsigned)a.Hkv, (unsigned)zf), dim3(256), 0, st, a, 0, 0, 0, 0);
+  RAI_TRY(launch_check("kv_attention_join"));
   if (odd.src) {
     const int64_t blocks = (a.N * a.Hq * odd.D + 255) / 256;
     hipLaunchKernelGGL((k_kv_rows_narrow<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, back);
