@@ -209,7 +209,8 @@ template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, c
     if (pass == 0) {
       total = at;
       if (d.workers) {
-        out->share = max((int64_t)((double)total * d.per_worker) + 1, (int64_t)d.least * kUnits);   // times the workers: no less than the total
+        const int64_t even = (int64_t)((double)total * d.per_worker);
+        out->share = max(even + 1 + (even >> 50), (int64_t)d.least * kUnits);   // times the workers: no less than the total
         u = worker * out->share;
         if (threadIdx.x == 0) d.join[(int64_t)kvh * d.workers + worker].first = -1;
       }
@@ -1107,7 +1108,8 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
   RAI_REQUIRE(window >= 0, RAI_ERR_BAD_ARG, "kv_attention: window %d", window);
   const rai_hip_tensor *ins[] = {q, tables, starts, lens, k, v, k_scale, v_scale};
   for (const rai_hip_tensor *i : ins) RAI_REQUIRE(!overlap(i, out), RAI_ERR_BAD_ARG, "kv_attention: out lies over an input");
-  RAI_REQUIRE(N * (Hq / c.heads) / 16 + R < (int64_t)1 << 23, RAI_ERR_UNSUPPORTED, "kv_attention: %lld rows of %lld heads to a key head and %lld requests", (long long)N, (long long)(Hq / c.heads), (long long)R);
+  RAI_REQUIRE((N * (Hq / c.heads) / 16 + R) * c.heads < (int64_t)1 << 23, RAI_ERR_UNSUPPORTED, "kv_attention: %lld rows of %lld heads over %d and %lld requests are more than 2^23 tiles", (long long)N,
+              (long long)Hq, c.heads, (long long)R);
   hipStream_t st = stream_of(dev);
   if (!st) return RAI_ERR_HIP;
   if (N == 0 || R == 0) return RAI_OK;

@@ -150,3 +150,8 @@ def test_attention_refuses(want, over):
 def test_attention_refuses_an_output_over_an_input():
     q = t("bf16", 5, 4, 60)
     assert attention(q=q, out=q) == ARG
+
+
+def test_attention_refuses_more_tiles_than_a_launch_holds():
+    """2^22 tiles of a head, of two heads."""
+    assert attention(q=t("bf16", 1 << 25, 4, 60), out=t("bf16", 1 << 25, 4, 60)) == UNSUPPORTED
