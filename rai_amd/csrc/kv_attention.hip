@@ -23,8 +23,9 @@ struct KvKind {
   float *part_m, *part_l;        // their maxima and sums of weights
   struct KvJoin *join;           // [Hkv * workers]
 };
-// The tile whose last part is a worker's first: workers first .. the worker itself have its parts.
-struct KvJoin {
+// The tile whose last part is a worker's first: workers first .. the worker itself have its parts.  (Whole 16 bytes: behind these of one kind lie the sums of the other,
+// which are written 16 bytes at a time.)
+struct alignas(16) KvJoin {
   int first;                     // -1: none
   int place;                     // which of the first worker's two parts
   int start, column, columns;    // the tile's request's first row, its first column and how many it has
@@ -1004,6 +1005,7 @@ template <typename T, int VT, int NC> struct KvShares {
     workers = steps <= kv_alone(NC, 2 * tiles >= slots) ? 0 : n < 1 ? 1 : (int)n;
     parts = 2ll * QT * a.Hkv * workers;
   }
+  static_assert(QT * sizeof(float) % 16 == 0 && sizeof(KvJoin) % 16 == 0, "whole 16 bytes of scratch");
   size_t bytes(const KvAttnArgs &a) const { return (size_t)(parts * (a.features + 2) * 4) + (size_t)a.Hkv * workers * sizeof(KvJoin); }
   KvKind kind(const KvAttnArgs &a, int which, void *ws) const {
     KvKind d;
@@ -1049,6 +1051,7 @@ template <typename T, int FMT, int VT> static int launch_kv_attention(hipStream_
   }
   a.few = few.kind(a, wide ? 1 : 0, base + 2 * rows);
   if (wide) a.many = many.kind(a, 2, base + 2 * rows + of_few);
+  RAI_REQUIRE(((uintptr_t)a.few.part | (uintptr_t)a.many.part) % 16 == 0, RAI_ERR_UNSUPPORTED, "kv_attention: scratch of %zu and %zu bytes off 16", of_few, of_many);
   dim3 grid;
   RAI_TRY(grid_of_blocks((int64_t)a.few.blocks + a.many.blocks, 256, &grid));
   RAI_REQUIRE(grid.y == 1, RAI_ERR_UNSUPPORTED, "kv_attention: %d blocks", a.few.blocks + a.many.blocks);
