@@ -289,35 +289,39 @@ template <int VT> struct KvFeatures {
 };
 template <typename T, int VT, int NC, bool TOGETHER>
 __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<NC> &k, kv_bf16x8 (&qf)[NC][KvFeatures<VT>::KS][KvTerms<T>::n]) {
-  constexpr int TERMS = KvTerms<T>::n, KS = KvFeatures<VT>::KS;
-  struct alignas(16) Eight { T v[8]; } all[NC][KS];
-  // (no branch: lanes without these features take others and put zeros in their place)
-  bool there[KS];
+  constexpr int TERMS = KvTerms<T>::n, KS = KvFeatures<VT>::KS, WORDS = 2 * sizeof(T);
+  struct alignas(16) Eight { uint32_t w[WORDS]; } all[NC][KS];
+  // Lanes without these features take others and clear them by a mask.  No branch, and none for the compiler to make of a condition (it does not know
+  // what the mask holds): in front of the end of one it has put copies of registers that belong behind it, so that they were made for some lanes only and
+  // addresses were lost.
+  uint32_t keep[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
-    there[s] = d0 < a.D;
+    keep[s] = d0 < a.D ? 0xffffffffu : 0u;
+    asm volatile("" : "+v"(keep[s]));
 #pragma unroll
-    for (int c = 0; c < NC; ++c) all[c][s] = *reinterpret_cast<const Eight *>((const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head + (there[s] ? d0 : 0));
+    for (int c = 0; c < NC; ++c) all[c][s] = *reinterpret_cast<const Eight *>((const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head + (d0 & (int)keep[s]));
   }
   if (TOGETHER) __builtin_amdgcn_sched_barrier(0);   // all on their way before the first is waited for
+  const uint32_t turn = sizeof(T) == 2 ? a.turn : a.turn & 0x80000000u;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const Eight e = all[c][s];
-      if constexpr (TERMS == 1) {
-        kv_u32x4 x = __builtin_bit_cast(kv_u32x4, e);
+      Eight e = all[c][s];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = there[s] ? x[j] ^ a.turn : 0u;
-        qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, x);
+      for (int j = 0; j < WORDS; ++j) e.w[j] = (e.w[j] ^ turn) & keep[s];
+      if constexpr (TERMS == 1) {
+        qf[c][s][0] = __builtin_bit_cast(kv_bf16x8, e);
       } else {
-        const float sign = a.turn ? -1.f : 1.f;
+        struct Values { T v[8]; };
+        const Values x = __builtin_bit_cast(Values, e);
         union { kv_bf16x2 p[4]; kv_bf16x8 v; } u[TERMS];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           kv_bf16x2 t[TERMS];
-          kv_split2<TERMS>(there[s] ? (float)Scalar<T>::load(&e.v[2 * j]) * sign : 0.f, there[s] ? (float)Scalar<T>::load(&e.v[2 * j + 1]) * sign : 0.f, t);
+          kv_split2<TERMS>((float)Scalar<T>::load(&x.v[2 * j]), (float)Scalar<T>::load(&x.v[2 * j + 1]), t);
 #pragma unroll
           for (int i = 0; i < TERMS; ++i) u[i].p[j] = t[i];
         }
