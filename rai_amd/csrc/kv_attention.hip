@@ -299,7 +299,7 @@ __device__ __forceinline__ void kv_queries(const KvAttnArgs &a, const KvColumns<
   for (int s = 0; s < KS; ++s) {
     const int d0 = KvFeatures<VT>::of_product(s, (threadIdx.x & 63) >> 4);
     keep[s] = d0 < a.D ? 0xffffffffu : 0u;
-    asm volatile("" : "+v"(keep[s]));
+    asm("" : "+v"(keep[s]));
 #pragma unroll
     for (int c = 0; c < NC; ++c) all[c][s] = *reinterpret_cast<const Eight *>((const T *)a.q + (int64_t)k.rows[c] * a.q_row + (int64_t)k.heads[c] * a.q_head + (d0 & (int)keep[s]));
   }
