@@ -402,7 +402,7 @@ int rai_hip_kv_append(int dev, const rai_hip_tensor *new_k, const rai_hip_tensor
  * Pages of a shared prefix may stand in many tables.  A page number that is not there hides its tokens, and counts as an index error, as
  * does a length past M * page, of which the first M * page tokens are seen.  Scales are positive.  Codes that are NaN (no
  * rai_hip_kv_append writes one) may reach rows that do not see their token.  Products are exact and sums in f32; weights are rounded to 16
- * significant bits or more, to 8 for bf16 rows of batches that fill the device many times over.  Long contexts are cut over blocks: their sums go
+ * significant bits or more.  Long contexts are cut over blocks: their sums go
  * through the device's scratch, of a size that does not grow with the batch, as do rows off 16-byte boundaries and heads whose
  * features are in no whole eights, of one that does. */
 int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_hip_tensor *tables, const rai_hip_tensor *starts, const rai_hip_tensor *lens,

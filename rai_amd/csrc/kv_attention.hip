@@ -72,9 +72,9 @@ template <int FMT> __device__ __forceinline__ kv_bf16x8 kv_unpack(uint32_t lo, u
 __device__ __forceinline__ kv_u32x4 fetch_once(const uint8_t *p) { return __builtin_nontemporal_load(reinterpret_cast<const kv_u32x4 *>(p)); }
 
 // How many bf16 hold a value of type T: products with codes are then exact, so f16 and f32 rows lose nothing on the bf16 matrix instructions.  The softmax's
-// weights are rounded to as many, of tiles of few columns to two at least: with one, results of bf16 rows are off by 0.0022 to 0.0024 of their size, with two by 0.0016
-// to 0.0017, which is the output's own rounding, and a step that waits for memory has room for it (64 requests 53 us either way).  Tiles of many
-// columns, bound by instructions, keep one (prompts of 2300 rows 85 us, with two 100).
+// weights are rounded to as many, to two at least: to 16 significant bits in every tile, so that neither the batch nor the width of its tables decides how far a
+// result is off.  With one, results of bf16 rows are off by 0.0022 to 0.0024 of their size, with two by 0.0016 to 0.0017, which is the output's own rounding.  It
+// costs nothing where a step waits for memory (64 requests 51 us either way), but an eighth where instructions bound it: prompts of 2300 rows 87 us for 77.
 template <typename T> struct KvTerms;
 template <> struct KvTerms<bf16_raw> { static constexpr int n = 1, weights = 2; };
 template <> struct KvTerms<f16_raw> { static constexpr int n = 2, weights = 2; };
@@ -680,7 +680,7 @@ __device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
 template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
   typedef KvFeatures<VT> Fe;
-  constexpr int TERMS = KvTerms<T>::n, WEIGHTS = TERMS, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
+  constexpr int TERMS = KvTerms<T>::n, WEIGHTS = KvTerms<T>::weights, QT = 32 * NC, KS = Fe::KS, BYTES = 64 * 16 * VT, LOADS = (2 * VT + 3) / 4;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = w >> 1;
   const int per_head = d.blocks / a.Hkv, place = kv_block(d, block), kvh = place / per_head, worker = place % per_head;
   KvWork k;
