@@ -128,7 +128,7 @@ def attention(q, tables, starts, lens, form, k, v, k_scale, v_scale, page, scale
     out, spread, slip = np.zeros((N, Hq, D)), np.zeros((N, Hq, D)), np.zeros((N, Hq, 1))
     G = Hq // k.shape[1]
     for r in range(len(lens)):
-        n, length = int(starts[r + 1] - starts[r]), max(int(lens[r]), 0)
+        n, length = int(starts[r + 1] - starts[r]), min(max(int(lens[r]), 0), tables.shape[1] * page)   # what its table holds
         if n == 0 or length == 0:
             continue
         ids = [int(t) for t in tables[r, :-(-length // page)]]

@@ -40,7 +40,8 @@ struct KvAttnArgs {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   uint32_t pages;
-  int dev, R, Hq, Hkv, G, D, features, page_shift, window;
+  int dev, R, Hq, Hkv, G, D, features, page_shift;
+  int64_t window;
   float scale_log2;              // |scale| * log2(e)
   uint32_t turn;                 // the signs of two bf16 where the scale is negative
   double per_group;              // 1 / G
@@ -136,20 +137,22 @@ constexpr int kv_extra = 6;
 constexpr int kUnits = 16 * kStep;   // of a step
 struct KvRequest {
   int start, n, tiles;           // first row, new tokens
-  int len, first;                // length, cut to its table's; position of the first new token
+  int len;                       // length, cut to its table's
+  int64_t first;                 // position of the first new token, of the whole length
 };
 __device__ __forceinline__ int64_t kv_base(const KvAttnArgs &a, const KvRequest &q) { return 16ll * min(max(q.len - q.n, 0), a.reach); }
 __device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvKind &d, const KvRequest &q, int64_t tile) { return kv_base(a, q) + d.extra + (int64_t)d.each * (tile + 1); }
 // of the tiles before `tile`
 __device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const KvKind &d, const KvRequest &q, int64_t tile) { return tile * (kv_base(a, q) + d.extra) + d.each * (tile * (tile + 1) / 2); }
 
+constexpr int64_t kKvFar = (int64_t)1 << 40;   // past every table and window
 template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, const KvKind &d, int r) {
   KvRequest q;
   const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), said = a.lens[r], most = a.M << a.page_shift;
   q.start = (int)start;
   q.n = (int)(min(max(a.starts[r + 1], start), a.N) - start);
   q.len = (int)min(max(said, (int64_t)0), most);
-  q.first = (int)min(max(said, -(1ll << 30)), most) - q.n;
+  q.first = min(max(said, -kKvFar), kKvFar) - q.n;
   const int columns = q.n * a.G;
   q.tiles = d.which == 1 ? columns > 0 && columns <= 16 : d.which == 2 && columns <= 16 ? 0 : (columns + QT - 1) / QT;
   return q;
@@ -201,7 +204,7 @@ template <int QT> __device__ __forceinline__ bool kv_deal(const KvAttnArgs &a, c
         out->req.start = __builtin_amdgcn_readlane(x.start, f);
         out->req.n = __builtin_amdgcn_readlane(x.n, f);
         out->req.len = __builtin_amdgcn_readlane(x.len, f);
-        out->req.first = __builtin_amdgcn_readlane(x.first, f);
+        out->req.first = lane_of(x.first, f);
         out->req.tiles = __builtin_amdgcn_readlane(x.tiles, f);
         break;
       }
@@ -252,13 +255,15 @@ template <int QT> __device__ __forceinline__ bool kv_next(const KvAttnArgs &a, c
   }
   return true;
 }
-// Which keys the tokens of a request see: of token i, oldest(i) .. newest(i).
+// Which keys the tokens of a request see: of token i, oldest(i) .. newest(i), none where the oldest is the newer.
 struct KvSeen {
-  int first, len, window;
+  int64_t first, window;
+  int len;
   double per_group;
   __device__ __forceinline__ int token(int x) const { return (int)(((double)x + 0.5) * per_group); }   // of column x
-  __device__ __forceinline__ int newest(int i) const { return min(max(first + i, -1), len - 1); }
-  __device__ __forceinline__ int oldest(int i) const { return max(max(first + i, -1) - window + 1, 0); }
+  __device__ __forceinline__ int64_t at(int i) const { return max(first + i, (int64_t)-1); }
+  __device__ __forceinline__ int newest(int i) const { return (int)min(at(i), (int64_t)len - 1); }
+  __device__ __forceinline__ int oldest(int i) const { return (int)min(max(at(i) - window + 1, (int64_t)0), (int64_t)len); }
 };
 // Columns of a tile, 16 to a lane group's place in NC: row of q and head, and what they see.
 template <int NC> struct KvColumns {
@@ -530,7 +535,7 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
   for (bool first = true;; first = false) {
     const int64_t size = kv_units(a, d, k.req, k.tile), to = min(size, k.from + k.left);
     const int len = k.req.len, columns = k.req.n * a.G;
-    const KvSeen see = {k.req.first, len, a.window, a.per_group};
+    const KvSeen see = {k.req.first, a.window, len, a.per_group};
     const KvColumns<1> cols = kv_columns<1>(a, k.req, see, kvh, k.tile * QT, columns);
     // of the tile's first and last token: every live column sees lo_last .. hi_first, none sees outside lo_first .. hi_last
     const int i_first = see.token(k.tile * QT), i_last = see.token(min((k.tile + 1) * QT, columns) - 1);
@@ -721,7 +726,7 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
   for (bool first = true;; first = false) {
     const int64_t size = kv_units(a, d, k.req, k.tile), to = min(size, k.from + k.left);
     const int len = k.req.len, columns = k.req.n * a.G;
-    const KvSeen see = {k.req.first, len, a.window, a.per_group};
+    const KvSeen see = {k.req.first, a.window, len, a.per_group};
     const int x0 = k.tile * QT, xw = x0 + (w & 1) * 16 * NC;
     const KvColumns<NC> cols = kv_columns<NC>(a, k.req, see, kvh, xw, columns);
     // what the tile's first and last token see, for the steps; and this wave's, for what it may skip or need not mask
@@ -1136,7 +1141,7 @@ extern "C" int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_
   a.pages = (uint32_t)(M == 0 ? 0 : c.pages < (int64_t)UINT32_MAX ? c.pages : (int64_t)UINT32_MAX);
   a.R = (int)R; a.Hq = (int)Hq; a.Hkv = c.heads; a.G = (int)(Hq / c.heads); a.D = (int)D;
   a.features = c.features; a.page_shift = c.page_shift;
-  a.window = window > 0 ? window : INT32_MAX;
+  a.window = window > 0 ? window : 2 * kKvFar;
   a.reach = window > 0 && window < INT32_MAX - kStep ? window + kStep : INT32_MAX;
   a.per_group = 1.0 / a.G;
   // rows off 16-byte boundaries, and heads of features in no whole eights, go through rows of the cache's features

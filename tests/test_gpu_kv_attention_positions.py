@@ -1,0 +1,34 @@
+"""Attention over the paged cache: where rows sit, and what they see, in calls that go past a table or past the batch's rows."""
+import numpy as np
+import pytest
+
+from oracle import kv_cache as O
+from rai_amd import ops
+from tests.kv_models import dev, rows
+from tests.kv_steps import Seen, want
+from tests.util import down, up
+
+pytestmark = pytest.mark.gpu
+
+
+def check(b, q, dt, scale, window=0):
+    ops.index_errors()
+    got = down(b.cache().attention(up(q, dt), dev(b.tables, "u32"), dev(b.starts, "i64"), dev(b.lens, "i64"), scale, window)).astype(np.float64)
+    exact, bound = want(b, q, dt, scale, window)
+    over = np.abs(got - exact) / np.maximum(bound, 1e-300)
+    assert (np.abs(got - exact) <= bound).all(), f"{over.max()} of the bound at {np.unravel_index(over.argmax(), over.shape)}"
+    return got
+
+
+@pytest.mark.parametrize("window", [0, 1, 16, 100, 2 ** 31 - 1])
+@pytest.mark.parametrize("more", [1, 5, 40, 150, 10 ** 12, 2 ** 62])
+@pytest.mark.parametrize("dt,new,heads", [("bf16", [1, 9, 3], 8), ("f32", [9, 130, 1], 8), ("bf16", [130, 128, 60], 40)])
+def test_a_length_past_the_table(hip, dt, new, heads, more, window):
+    """Rows keep the positions that the length gives them, and see the tokens that the table holds."""
+    rng = np.random.default_rng(heads + window % 1000)
+    b = Seen(rng, [192, 160, 192], new, 16, 1, 64, "e4m3", 1, table=12)
+    b.lens[:] = [192 + more, 160, 192 + more]
+    got = check(b, rows(rng, (b.N, heads, 64), dt), dt, 0.1, window)
+    assert ops.index_errors() == 2
+    if 0 < window <= more - new[0]:
+        assert (got[:new[0]] == 0).all()
