@@ -128,13 +128,14 @@ def attention(q, tables, starts, lens, form, k, v, k_scale, v_scale, page, scale
     out, spread, slip = np.zeros((N, Hq, D)), np.zeros((N, Hq, D)), np.zeros((N, Hq, 1))
     G = Hq // k.shape[1]
     for r in range(len(lens)):
-        n, length = int(starts[r + 1] - starts[r]), min(max(int(lens[r]), 0), tables.shape[1] * page)   # what its table holds
-        if n == 0 or length == 0:
+        lo, hi = (min(max(int(x), 0), N) for x in starts[r:r + 2])      # of its rows those that are there
+        length = min(max(int(lens[r]), 0), tables.shape[1] * page)      # of its tokens those that its table holds
+        if hi <= lo or length == 0:
             continue
         ids = [int(t) for t in tables[r, :-(-length // page)]]
         there = np.repeat([t < k.shape[0] for t in ids], page)[:length]
         ids = [t if t < k.shape[0] else 0 for t in ids]
-        p = int(lens[r]) - n + np.arange(n)[:, None]
+        p = int(lens[r]) - int(starts[r + 1]) + np.arange(lo, hi)[:, None]
         j = np.arange(length)[None]
         hidden = (j > p) | ~there
         if window:
@@ -143,14 +144,14 @@ def attention(q, tables, starts, lens, form, k, v, k_scale, v_scale, page, scale
             kk = kd[ids, h // G].reshape(-1, D)[:length]
             vv = np.where(there[:, None], vd[ids, h // G].transpose(0, 2, 1).reshape(-1, D)[:length], 0.0)
             kk = np.where(there[:, None], kk, 0.0)
-            x = q[starts[r]:starts[r + 1], h]
+            x = q[lo:hi, h]
             s = np.where(hidden, -np.inf, x @ kk.T * scale)
             top = np.max(s, 1, keepdims=True)
             w = np.where(hidden, 0.0, np.exp(s - np.where(np.isfinite(top), top, 0.0)))
             total = w.sum(1, keepdims=True)
             w = np.divide(w, total, out=np.zeros_like(w), where=total > 0)
-            out[starts[r]:starts[r + 1], h] = w @ vv
-            spread[starts[r]:starts[r + 1], h] = w @ np.abs(vv)
+            out[lo:hi, h] = w @ vv
+            spread[lo:hi, h] = w @ np.abs(vv)
             size = np.where(hidden, 0.0, np.abs(x) @ np.abs(kk).T * abs(scale))
-            slip[starts[r]:starts[r + 1], h] = size.max(1, keepdims=True)
+            slip[lo:hi, h] = size.max(1, keepdims=True)
     return out, spread, slip

@@ -138,7 +138,7 @@ constexpr int kUnits = 16 * kStep;   // of a step
 struct KvRequest {
   int start, n, tiles;           // first row, new tokens
   int len;                       // length, cut to its table's
-  int64_t first;                 // position of the first new token, of the whole length
+  int64_t first;                 // position of the first row, by the whole length
 };
 __device__ __forceinline__ int64_t kv_base(const KvAttnArgs &a, const KvRequest &q) { return 16ll * min(max(q.len - q.n, 0), a.reach); }
 __device__ __forceinline__ int64_t kv_units(const KvAttnArgs &a, const KvKind &d, const KvRequest &q, int64_t tile) { return kv_base(a, q) + d.extra + (int64_t)d.each * (tile + 1); }
@@ -148,11 +148,13 @@ __device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs &a, const Kv
 constexpr int64_t kKvFar = (int64_t)1 << 40;   // past every table and window
 template <int QT> __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs &a, const KvKind &d, int r) {
   KvRequest q;
-  const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), said = a.lens[r], most = a.M << a.page_shift;
+  const int64_t start = min(max(a.starts[r], (int64_t)0), a.N), end = a.starts[r + 1], said = a.lens[r], most = a.M << a.page_shift;
   q.start = (int)start;
-  q.n = (int)(min(max(a.starts[r + 1], start), a.N) - start);
+  q.n = (int)(min(max(end, start), a.N) - start);
   q.len = (int)min(max(said, (int64_t)0), most);
-  q.first = min(max(said, -kKvFar), kKvFar) - q.n;
+  int64_t first;                 // its rows end with the length, also where some are not there
+  if (__builtin_sub_overflow(said, end, &first)) first = said < 0 ? -kKvFar : kKvFar;
+  q.first = min(max(first, -kKvFar), kKvFar) + start;
   const int columns = q.n * a.G;
   q.tiles = d.which == 1 ? columns > 0 && columns <= 16 : d.which == 2 && columns <= 16 ? 0 : (columns + QT - 1) / QT;
   return q;

@@ -32,3 +32,17 @@ def test_a_length_past_the_table(hip, dt, new, heads, more, window):
     assert ops.index_errors() == 2
     if 0 < window <= more - new[0]:
         assert (got[:new[0]] == 0).all()
+
+
+@pytest.mark.parametrize("window", [0, 30])
+@pytest.mark.parametrize("dt,heads", [("bf16", 8), ("f32", 40)])
+@pytest.mark.parametrize("rows_there", [1, 39, 81, 100, 160, 199])
+def test_requests_whose_rows_are_not_all_there(hip, rows_there, dt, heads, window):
+    """As after a plan that refused requests for want of rows: starts go on past the batch's rows, and those that are there sit where they would."""
+    rng = np.random.default_rng(rows_there + heads)
+    b = Seen(rng, [200, 130, 190], [40, 40, 120], 16, 1, 64, "int8", 1, table=16)
+    check(b, rows(rng, (rows_there, heads, 64), dt), dt, 0.1, window)
+    assert ops.index_errors() == 0
+    b.starts[3] = 2 ** 62
+    b.lens[2] = 2 ** 62 + 3 - rows_there   # positions as far as numbers go
+    check(b, rows(rng, (rows_there, heads, 64), dt), dt, 0.1, window)
