@@ -592,7 +592,7 @@ template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(co
         const KvScales coming = kv_scales(a, of_v, kvh);
         const int key0 = st * kStep + 16 * g;   // this lane group's first
         const bool gone = key0 < len && !scales.there;
-        missing |= gone;
+        missing |= gone && key0 + 15 >= lo_first && key0 <= hi_last;   // some row of the tile would see it
         if ((st + 1) * kStep > len || __any(gone)) {
           // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be
           const int valid = scales.there ? min(len - key0, 16) : 0;
@@ -791,7 +791,7 @@ template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void k
         load(next, entries, lds_at + (b ^ 1) * 4 * BYTES);
         ask(min(st0 + 4, last), entries, e_scales);
         const bool gone = st < s_end && key0 < len && !scales.there;
-        missing |= gone;
+        missing |= gone && key0 + 15 >= lo_first && key0 <= hi_last;   // some row of the tile would see it
         uint8_t *const kt = lds + (b * 4 + half * 2) * BYTES, *const vt = kt + BYTES;
         if (st < s_end && ((st + 1) * kStep > len || __any(gone))) {
           // codes behind the context may be anything; their weight is zero, and zero times a NaN would not be.  (Each wave does it for itself: the

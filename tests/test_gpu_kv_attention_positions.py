@@ -46,3 +46,24 @@ def test_requests_whose_rows_are_not_all_there(hip, rows_there, dt, heads, windo
     b.starts[3] = 2 ** 62
     b.lens[2] = 2 ** 62 + 3 - rows_there   # positions as far as numbers go
     check(b, rows(rng, (rows_there, heads, 64), dt), dt, 0.1, window)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("window", [1, 16, 50, 100])
+@pytest.mark.parametrize("dt,heads,new", [("bf16", 8, [1, 1, 1]), ("f32", 8, [1, 33, 20]), ("bf16", 40, [110, 120, 30])])
+def test_pages_that_a_window_has_left(hip, dt, heads, new, window, page):
+    """Entries of pages that no row sees may be anything; those of pages of which a row would see one token count."""
+    rng = np.random.default_rng(window + heads)
+    b = Seen(rng, [400, 257, 300], new, page, 1, 64, "e4m3", 1)
+    q = rows(rng, (b.N, heads, 64), dt)
+    oldest = [t - n - window + 1 for t, n in zip(b.total, new)]
+    for r, o in enumerate(oldest):
+        b.tables[r, :o // page] = 2 ** 32 - 1 - np.arange(o // page)
+    check(b, q, dt, 0.1, window)
+    assert ops.index_errors() == 0
+    for r in range(3):
+        kept = b.tables[r, oldest[r] // page]
+        b.tables[r, oldest[r] // page] = b.pages
+        check(b, q, dt, 0.1, window)
+        assert ops.index_errors() > 0, r
+        b.tables[r, oldest[r] // page] = kept
