@@ -400,9 +400,11 @@ int rai_hip_kv_append(int dev, const rai_hip_tensor *new_k, const rai_hip_tensor
  * [N, Hq, D] contiguous in q's dtype; rows that belong to no request are left as they are.
  *   tables u32 [R, M] (unit stride along M), starts i64 [R + 1] not falling, lens i64 [R] (after rai_hip_kv_plan: out_lens)
  * Pages of a shared prefix may stand in many tables.  A page number that is not there hides its tokens, and counts as an index error where a row would
- * see one of them (so that pages which a window has left behind may be given away), as does a length past M * page: its rows sit where it says and see what they would of the first M * page tokens.  Scales are positive.  Codes that are NaN (no
- * rai_hip_kv_append writes one) may reach rows that do not see their token.  Products are exact and sums in f32; weights are rounded to 16
- * significant bits or more.  Long contexts are cut over blocks: their sums go
+ * see one of them (so that pages which a window has left behind may be given away), as does a length past M * page: its rows sit where it says and see
+ * what they would of the first M * page tokens.  Scales are positive and no subnormal numbers; values are below 2^80, sums of them times weights being in
+ * f32 before they are divided by the weights' sum.  Codes that are NaN (no rai_hip_kv_append writes one) may reach rows that do not see their token.
+ * Products are exact and sums in f32; weights are rounded to 16 significant bits or more.  Long contexts are cut over blocks, as the width of the
+ * tables and not the lengths have it, so that the order of sums, and last bits with it, may differ from width to width; their sums go
  * through the device's scratch, of a size that does not grow with the batch, as do rows off 16-byte boundaries and heads whose
  * features are in no whole eights, of one that does. */
 int rai_hip_kv_attention(int dev, const rai_hip_tensor *q, const rai_hip_tensor *tables, const rai_hip_tensor *starts, const rai_hip_tensor *lens,

@@ -114,26 +114,28 @@ constexpr int kStep = 64;                      // keys of a step
 
 // Blocks of a kernel that a CU holds.
 constexpr int kv_blocks(int vt, int nc, int terms) { return vt > 8 || (nc > 1 && terms > 1 && vt > 4) ? 1 : nc > 1 || vt > 5 || terms > 1 ? 2 : 3; }
-// Tiles of up to so many steps are not shared between workers; `full`: where tiles as they are keep half the card busy.  Measured, whole against shared: of
-// few columns, 16 requests of up to 1200 keys over 8 heads (19 steps) 16 us against 22 and of up to 2048 over 32 heads (32, full) 26 against 33, but one of
-// 2048 over 32 heads (not full) 19 against 14, and 16 of up to 4000 (63, full) 40 against 38; of many, a window of 512 keys (10) 38 against 42, 16 chunks of up
-// to 256 behind up to 700 (11) 28 against 43, 8 of up to 1024 with nothing before (16) 56 against 62, but a window of 1024 (18) 57 against 51.
+// Tiles of up to so many steps, which a table has room for, are not shared between workers; `full`: where tiles as they are keep half the card busy.  Measured, whole against
+// shared: of few columns, 16 requests of up to 1200 keys over 8 heads (19 steps) 16 us against 18 and of up to 2048 over 32 heads (32, full) 24 against 27, but one
+// of 2048 over 32 heads (not full) 18 against 13, and 16 of up to 4000 (63, full) 39 against 33; of many, 16 chunks of up to 256 behind up to 700 (11) 30 against 43, 8
+// of up to 1024 with nothing before (16) 59 against 63, but a window of 1024 (18) 56 against 43 and one of 512 (10) 37 against 33, which goes through tiles of few.
 constexpr int kv_alone(int nc, bool full) { return nc ? 16 : full ? 40 : 24; }
 // Requests of many columns go through tiles of few as well where all tiles of 16 find room on the card at once and have up to so many steps for each place there: four
 // waves then share a tile's steps, and no tile waits for another.  So against tiles of many: 9 chunks of up to 37 in a window of 512 keys (f32, 256 features, 4 steps a
-// place) 29 us against 38, 640 rows behind nothing (10) 17 against 24, 4 chunks of up to 64 behind up to 4000 (15) 26 against 47, 16 of up to 64 behind
-// up to 2000 (f32, 28) 36 against 43; beyond, 300 rows behind 5000 (35) 50 against 43, 16 chunks of up to 64 behind up to 4000 (56) 49 against 43.
+// place) 25 us against 37, 640 rows behind nothing (10) 16 against 23, 4 chunks of up to 64 behind up to 4000 (15) 26 against 36, 16 of up to 64 behind
+// up to 2000 (f32, 28) 36 against 39; beyond, 300 rows behind 5000 (35) 47 against 45, 16 chunks of up to 64 behind up to 4000 (56) 45 against 41.
 constexpr int kv_small = 32;
-// Steps of a share at least.  Of few columns with 8, with 4 and with 16: one request of 100000 keys 30, 47 and 23 us, of 8000 15, 13 and 19, four of 4000 over 8 heads 17, 19 and 22;
-// of many with 2, 1 and 4: 700 rows behind 8000 keys 75, 76 and 77.
+// Steps of a share at least.  Of few columns with 8, with 4 and with 16: one request of 100000 keys 29, 43 and 23 us, of 8000 14, 13 and 17, four of 4000 over 8 heads 16, 19 and 20;
+// of many with 2, 1 and 4: 700 rows behind 8000 keys 84 to 86.
 constexpr int kv_least(int nc) { return nc ? 2 : 8; }
-// Steps that a tile's beginning and end take as long as.  Prompts of 2300 rows 105 us with 3, 100 with 6, 105 with 9, 110 with 12; one request of 8000 keys 14.5 us
-// with 6, 19 with 12.
+// Steps that a tile's beginning and end take as long as.  Prompts of 2300 rows 94 us with 3, 87 with 6, 93 with 9, 94 with 12; sixteen of them 275, 241, 246 and 257; one request of
+// 8000 keys 13 to 14 with any.
 constexpr int kv_extra = 6;
 
 // How the work of a key head is dealt out.  A tile of a request is as long as the keys that its last row sees, which grows evenly from tile to
 // tile, so that sums over tiles are known without a walk: in sixteenths of a key, tile t takes base + each * (t + 1), and `extra` for its beginning and end
-// (queries, first loads, the merge), which a worker that goes on to another tile pays again.
+// (queries, first loads, the merge), which a worker that goes on to another tile pays again.  These are prices, from which workers get their shares and tiles the seams between
+// them; the steps themselves are a tile's own.  Behind a window the work no longer grows and the price still does, so that shares of prompts longer than a window
+// of 1024 keys and more are uneven (8192 rows 275 us, without the window 368).
 constexpr int kUnits = 16 * kStep;   // of a step
 struct KvRequest {
   int start, n, tiles;           // first row, new tokens
@@ -511,7 +513,7 @@ __device__ __forceinline__ void kv_meet() {
 // fragments as they lie in registers, and every load of the cache is 16 bytes a lane, straight to registers.  Sixteen keys lie in one
 // page, so a lane group has one page and one scale of keys and of values.
 // Bound by memory and by what comes before the first step and behind the last: 64 requests of up to 16384 keys (236 MB) take 47 us and their join 4.7, 4.6 TB/s
-// in all where a read alone reaches 7.1 and a copy 4.7; a lone row over 777 keys takes 10 us, a chain of trips (lengths, table, keys, merge) and of code that is
+// in all where a read alone reaches 7.1 and a copy 4.7; a lone row over 777 keys takes 11 us, a chain of trips (lengths, table, keys, merge) and of code that is
 // run once.  A quarter of a wave reads sixteen keys' 16 bytes at a time: read as whole lines, at other results, the large case took 50 us.
 template <typename T, int VT> constexpr int kv_few_lds() { return 4 * VT * 64 * 16 + 4 * 2 * 64 * 4; }
 template <typename T, int FMT, int VT> __device__ __forceinline__ void kv_few(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
@@ -681,9 +683,9 @@ __device__ __forceinline__ void kv_to_lds(const uint8_t *from, uint32_t to) {
 // through LDS as codes, two buffers of two steps, one barrier for both: each byte of the cache reaches a CU once for 32 NC columns, and no
 // register holds what is on its way.  Keys lie in LDS in the order of the score tiles'
 // rows, their 16-byte pieces exchanged so that sixteen rows' reads spread over the banks; values as sixteen keys of a feature.
-// Bound by the instructions around the products: a step of 32 columns takes 64 matrix instructions (1024 clocks of a SIMD) and about 300 vector ones
-// (1600: codes to bf16 128, the softmax 160) and as many scalar ones in between, two waves to a SIMD.  Prompts of 2300 rows over up to 5000 keys, 34.6 GFLOP, take 77 us and
-// their join 9; sixteen of them 225 us, 530 TFLOP/s of the 1370 that a large product reaches.  Of the 77, 13 are workers' first and last trips.
+// Bound by the instructions around the products: a step of 32 columns takes 96 matrix instructions (1536 clocks of a SIMD) and about 370 vector ones
+// (1900: codes to bf16 128, the softmax 160, weights in two terms 80) and as many scalar ones in between, two waves to a SIMD.  Prompts of 2300 rows over up to 5000 keys,
+// 34.6 GFLOP, take 87 us with their join; sixteen of them 241 us, 495 TFLOP/s of the 1370 that a large product reaches.
 template <int VT> constexpr int kv_wide_lds() { return 8 * 64 * 16 * VT; }
 template <typename T, int FMT, int VT, int NC> __device__ __forceinline__ void kv_wide(const KvAttnArgs &a, const KvKind &d, int block, uint8_t *lds) {
   typedef KvFeatures<VT> Fe;
@@ -904,7 +906,7 @@ __global__ void __launch_bounds__(256, kv_blocks(VT, NC ? NC : 1, KvTerms<T>::n)
 }
 
 // The parts of tiles that workers share, to the output.  Blocks for each worker that had a tile's last part, over the tile's columns: a wave reads whole rows of
-// as many columns as fit it.  4.7 us behind 64 requests, 9 behind prompts of 2300 rows, most of it the launch and one trip.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
+// as many columns as fit it.  4.7 us behind 64 requests, 9 behind prompts of 2300 rows as a trace has it, most of it the launch and one trip.  PARTS: the block's waves take every fourth part each and meet in LDS (a context over many workers); else each its own columns.
 template <typename T, bool PARTS> __device__ __forceinline__ void kv_join(const KvAttnArgs &a, const KvKind &d, int QT, int worker, int kvh, int z, kv_f32x4 (*sums)[64], float (*stats)[2][64]) {
   const int64_t base = (int64_t)kvh * d.workers;
   const KvJoin j = d.join[base + worker];

@@ -113,7 +113,8 @@ __device__ __forceinline__ int first_above(const uint32_t *a, int n, uint32_t x)
 // pages taken + E_r .. + need_r - 1, E the sum of the needs before it; its new tokens are rows starts[r] .. of the batch, and each
 // page they touch gives a run (page, first slot, first row, rows).  Every block sums over all requests by itself (4096 at most: 64 KB
 // out of L2) rather than wait for another, keeps the three running sums in LDS, and then does its share of the runs, rows and table
-// entries, each of which finds its request by bisection there.  Bound by its chain of trips: lengths, sums, table entry, store; 64 requests take 5.3 us, 512 with
+// entries, each of which finds its request by bisection there.  Bound by its chain of trips: lengths read in each of three passes (a thread's requests
+// lie next to each other, so a wave's reads are spread), sums, bisection, table entry, store; 64 requests take 5.3 us, 512 with
 // 160 new rows each and tables of 1024 entries 9.2, a launch alone 4.2.
 __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(KvPlanArgs a) {
   extern __shared__ uint32_t plan_lds[];
@@ -305,8 +306,9 @@ template <int FMT> __device__ __forceinline__ uint32_t kv_rescale4(uint32_t x, f
 // writes whole 16-byte pieces of both features, without a trip through LDS.  What the first pass read stays in registers where a thread has
 // no more than four packs of keys or one piece of values, and is read again from the caches otherwise.
 // A unit owns its page and head alone: a run whose page an earlier run of the call names is refused.
-// Bound by memory, and by two passes over a unit where its values do not stay in registers: 16 prompts of up to 1300 rows of 8 heads of 128 features (61 MB) take 23 us,
-// 2.6 TB/s, a copy of as many bytes 13; 64 single tokens 5.8, a launch and a chain of trips.
+// Bound by vector instructions and by trips: 16 prompts of up to 1300 rows of 8 heads of 128 features (61 MB) take 23 us, 2.6 TB/s, a copy of as many bytes 13.  All of
+// a unit stays in registers there; 9.0 million vector instructions are 15 us of every SIMD's time, and the way from the run over its rows and their largest to the first
+// code, which the four waves of a SIMD hide in part, takes the rest.  64 single tokens 5.8 us, a launch and the same way once.
 template <typename T, int FMT, bool VEC, int WAVES>
 __global__ void __launch_bounds__(256) k_kv_append(KvAppendArgs a) {
   typedef KvFormat<FMT> Fm;
